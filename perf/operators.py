@@ -375,7 +375,7 @@ def _set_up(s):
         calls = [(lib.liger_kv8_compact, (by, at(s["live"]), at(s["moved_to"]), *space))]
     else:
         n = case["count"]
-        calls = [(lib.liger_kv8_free, (by, at(s["dst"]), n, *space)),
+        calls = [(lib.liger_kv8_free, (by, at(s["dst"]), n)),
                  (lib.liger_kv8_fork, (by, at(s["src"]), at(s["dst"]), at(s["lens"]), n, at(s["done"]), *space)),
                  (lib.liger_kv8_reserve, (by, at(s["dst"]), at(s["grown"]), n, at(s["roomy"]), *space))]
     return liger.check, calls, _pages_answer(s)
