@@ -9,6 +9,7 @@ compute entry point fails without a CUDA device.
 """
 from . import build, capi
 from .build import build_all, LIB_PATH
-from .capi import lib, check, LigerError, GemmArgs, ModelConfig, default_config
+from .capi import lib, check, LigerError, GemmArgs, Kv8Cache, Kv8AppendArgs, Kv8AttentionArgs, ModelConfig, default_config
 
-__all__ = ["capi", "build_all", "LIB_PATH", "lib", "check", "LigerError", "GemmArgs", "ModelConfig", "default_config"]
+__all__ = ["capi", "build_all", "LIB_PATH", "lib", "check", "LigerError", "GemmArgs", "Kv8Cache", "Kv8AppendArgs", "Kv8AttentionArgs",
+           "ModelConfig", "default_config"]

@@ -6,7 +6,8 @@ from .build import LIB_PATH
 
 LIGER_OK = 0
 EPI_STORE, EPI_GELU, EPI_GEGLU, EPI_QKV_SPLIT, EPI_RESIDUAL, EPI_SCATTER = 0, 1, 2, 3, 4, 5
-DEV_TIMEOUT = 1
+DEV_TIMEOUT, DEV_BAD_INDEX = 1, 2
+KV8_INT8, KV8_E4M3 = 0, 1
 
 
 class LigerError(RuntimeError):
@@ -27,6 +28,26 @@ class GemmArgs(C.Structure):
         ("scatter_comm", C.c_void_p), ("scatter_off", C.c_size_t),
         ("gather_comm", C.c_void_p), ("gather_channel", C.c_int),
     ]
+
+
+class Kv8Cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_pages", "v_pages", "k_scales", "v_scales", "page_table", "page_count", "page_refs")] + \
+               [(n, C.c_int) for n in ("layers", "num_pages", "kv_heads", "page_size", "scale_block", "head_dim", "type",
+                                       "slots", "max_pages")]
+
+
+class Kv8AppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "q_offsets", "slots", "positions")] + \
+               [(n, C.c_longlong) for n in ("batch_stride", "token_stride", "head_stride")] + \
+               [(n, C.c_int) for n in ("batch", "q_len", "total_tokens", "layer")]
+
+
+class Kv8AttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t)] + \
+               [(n, C.c_void_p) for n in ("q_offsets", "slots", "kv_lens")] + \
+               [(n, C.c_longlong) for n in ("q_batch_stride", "q_token_stride", "q_head_stride")] + \
+               [(n, C.c_int) for n in ("batch", "heads", "q_len", "total_tokens", "max_kv_len", "ldo", "layer", "causal")] + \
+               [("scale", C.c_float)]
 
 
 _P, _I, _F, _U32, _SZ = C.c_void_p, C.c_int, C.c_float, C.c_uint32, C.c_size_t
@@ -80,6 +101,15 @@ SIGNATURES = {
     "liger_attention_decode": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "liger_attention_decode_noalloc_max_bytes": (_SZ, []),
     "liger_attention_decode_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "liger_kv8_append": (_I, [C.POINTER(Kv8Cache), C.POINTER(Kv8AppendArgs), _P]),
+    "liger_kv8_attention_scratch_bytes": (_SZ, [C.POINTER(Kv8Cache), C.POINTER(Kv8AttentionArgs)]),
+    "liger_kv8_attention": (_I, [C.POINTER(Kv8Cache), C.POINTER(Kv8AttentionArgs), _P]),
+    "liger_kv8_pages_scratch_bytes": (_SZ, [C.POINTER(Kv8Cache), _I]),
+    "liger_kv8_reserve": (_I, [C.POINTER(Kv8Cache), _P, _P, _I, _P, _P, _SZ, _P]),
+    "liger_kv8_fork": (_I, [C.POINTER(Kv8Cache), _P, _P, _P, _I, _P, _P, _SZ, _P]),
+    "liger_kv8_free": (_I, [C.POINTER(Kv8Cache), _P, _I, _P]),
+    "liger_kv8_copy": (_I, [C.POINTER(Kv8Cache), _P, _P, _I, _P, _P, _SZ, _P]),
+    "liger_kv8_compact": (_I, [C.POINTER(Kv8Cache), _P, _P, _P, _SZ, _P]),
     "liger_layernorm": (_I, [_P, _P, _P, _P, _I, _I, _P]),
     "liger_add_bias_input_layernorm": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _P]),
     "liger_add_bias_gelu": (_I, [_P, _P, _I, _I, _P]),

@@ -1,0 +1,252 @@
+// Writing new keys and values into the paged 8-bit cache (liger_kv8_append), and the argument checks of its operators.
+//
+// A unit of work is one block of `scale_block` tokens of one head, keys or values.  Its threads hold all of the block's new
+// values in registers (64 per thread), so that the values are read once: the largest magnitude is found with integer maxima
+// on the fp16 bit patterns (for non-negative numbers the order of the patterns is the order of the values, and a NaN is above
+// infinity, so that it is not lost), then the codes are rounded and written.  The codes that a block already holds are only read
+// when its scale grows.
+#include "kv8.cuh"
+
+namespace liger {
+
+int kv8_check(const char* what, const liger_kv8_cache* c, int layer) {
+  if (!c) return set_error(LIGER_ERR_INVALID, "%s: cache is NULL", what);
+  if (!c->k_pages || !c->v_pages || !c->k_scales || !c->v_scales || !c->page_table)
+    return set_error(LIGER_ERR_INVALID, "%s: a pointer of the cache is NULL", what);
+  if (((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15u)
+    return set_error(LIGER_ERR_INVALID, "%s: k_pages / v_pages must be 16-byte aligned", what);
+  if (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales | (uintptr_t)c->page_table | (uintptr_t)c->page_count | (uintptr_t)c->page_refs) & 3u)
+    return set_error(LIGER_ERR_INVALID, "%s: scales and tables must be 4-byte aligned", what);
+  if (c->layers <= 0 || c->num_pages <= 0 || c->kv_heads <= 0 || c->slots <= 0 || c->max_pages <= 0)
+    return set_error(LIGER_ERR_INVALID, "%s: layers, num_pages, kv_heads, slots and max_pages must be positive", what);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return set_error(LIGER_ERR_UNSUPPORTED, "%s: head_dim %d (64 and 128 are implemented)", what, c->head_dim);
+  if (c->type != LIGER_KV8_INT8 && c->type != LIGER_KV8_E4M3) return set_error(LIGER_ERR_INVALID, "%s: type %d", what, c->type);
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+    return set_error(LIGER_ERR_UNSUPPORTED, "%s: page_size %d (powers of two from 16 to 256 are implemented)", what, c->page_size);
+  if (c->scale_block < 16 || c->scale_block > 128 || c->scale_block > c->page_size || (c->scale_block & (c->scale_block - 1)))
+    return set_error(LIGER_ERR_UNSUPPORTED, "%s: scale_block %d (powers of two from 16 to 128, at most page_size)", what, c->scale_block);
+  if (c->kv_heads > 65535 || (long long)c->max_pages * c->page_size > (1ll << 30))
+    return set_error(LIGER_ERR_UNSUPPORTED, "%s: kv_heads <= 65535, max_pages * page_size <= 2^30", what);
+  if (layer >= c->layers) return set_error(LIGER_ERR_INVALID, "%s: layer %d of %d", what, layer, c->layers);
+  return LIGER_OK;
+}
+
+static int log2_of(int x) {
+  int s = 0;
+  while ((1 << s) < x) ++s;
+  return s;
+}
+
+Kv8Layer kv8_layer(const liger_kv8_cache* c, int layer) {
+  const size_t blocks = (size_t)c->num_pages * c->kv_heads * (c->page_size / c->scale_block);
+  const size_t codes = (size_t)c->num_pages * c->kv_heads * c->page_size * c->head_dim;
+  Kv8Layer l;
+  l.k = (uint8_t*)c->k_pages + codes * layer;
+  l.v = (uint8_t*)c->v_pages + codes * layer;
+  l.ks = c->k_scales + blocks * layer;
+  l.vs = c->v_scales + blocks * layer;
+  l.table = c->page_table;
+  l.num_pages = c->num_pages;
+  l.kv_heads = c->kv_heads;
+  l.page_shift = log2_of(c->page_size);
+  l.block_shift = log2_of(c->scale_block);
+  l.slots = c->slots;
+  l.max_pages = c->max_pages;
+  return l;
+}
+
+int kv8_check_tokens(const char* what, const int* q_offsets, int batch, int q_len, int total_tokens, long long batch_stride,
+                     long long token_stride, long long head_stride) {
+  if (batch <= 0 || q_len <= 0) return set_error(LIGER_ERR_INVALID, "%s: batch and q_len must be positive", what);
+  if (batch > 65535 || q_len > (1 << 29)) return set_error(LIGER_ERR_UNSUPPORTED, "%s: batch <= 65535, q_len <= 2^29", what);
+  if (q_offsets ? total_tokens < 0 : (long long)batch * q_len > 0x7fffffffll)
+    return set_error(LIGER_ERR_INVALID, "%s: the number of tokens must be between 0 and 2^31 - 1", what);
+  if ((q_offsets == nullptr && batch_stride % 8) || token_stride % 8 || head_stride % 8)
+    return set_error(LIGER_ERR_INVALID, "%s: strides must be multiples of 8 elements", what);
+  if ((q_offsets == nullptr && batch_stride < 0) || token_stride < 0 || head_stride < 0)
+    return set_error(LIGER_ERR_INVALID, "%s: strides must not be negative", what);
+  if ((uintptr_t)q_offsets & 3u) return set_error(LIGER_ERR_INVALID, "%s: q_offsets must be 4-byte aligned", what);
+  return LIGER_OK;
+}
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+
+struct AppendParams {
+  Kv8Layer c;
+  Kv8Entries e;
+  const __half *k, *v;
+  const int* positions;
+  long long batch_stride, token_stride, head_stride;
+  int blocks;    // most blocks that one entry can touch
+  int unit;      // threads of a unit: a power of two, 32 .. 256
+  DeviceStatus* status;
+};
+
+// Grid: (units of an entry / units of a CTA, entries).  Units are ordered heads first, so that neighbouring warps read
+// neighbouring runs of the source's rows.
+template <int D, int TYPE, int U>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendParams p) {
+  constexpr int kPieces = D / 8;  // 16-byte pieces of a source row
+  __shared__ uint32_t s_max[kAppendThreads / 32];
+  const int b = blockIdx.y;
+  int n, row0;
+  const bool rows_ok = kv8_rows(p.e, b, n, row0);
+  const int slot = kv8_slot(p.e, b);
+  const int pos0 = __ldg(p.positions + b);
+  const bool lead = blockIdx.x == 0 && threadIdx.x == 0;
+  if (!rows_ok || n == 0) {
+    if (lead && !rows_ok) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend, b, 0);
+    return;
+  }
+  if (slot < 0 || slot >= p.c.slots || pos0 < 0 || (long long)pos0 + n > ((long long)p.c.max_pages << p.c.page_shift)) {
+    if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 1, b, (unsigned)slot);
+    return;
+  }
+  if (p.e.slots) {  // an earlier entry of the same slot has it
+    bool dup = false;
+    for (int j = threadIdx.x; j < b; j += kAppendThreads) dup |= __ldg(p.e.slots + j) == slot;
+    if (__syncthreads_or(dup)) {
+      if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 2, b, (unsigned)slot);
+      return;
+    }
+  }
+  const int t = threadIdx.x & (p.unit - 1);
+  const long long w = (long long)blockIdx.x * (kAppendThreads / p.unit) + threadIdx.x / p.unit;
+  const int head = (int)(w % p.c.kv_heads);
+  const int rest = (int)(w / p.c.kv_heads);
+  const int blk = rest % p.blocks, is_v = rest / p.blocks;
+  const int block0 = pos0 >> p.c.block_shift;            // the first block that is touched
+  const int start = (block0 + blk) << p.c.block_shift;   // this unit's first position
+  bool active = is_v < 2 && start < pos0 + n;
+  int page = -1;
+  if (active) {
+    page = __ldg(p.c.table + (size_t)slot * p.c.max_pages + (start >> p.c.page_shift));
+    if (page < 0 || page >= p.c.num_pages) {
+      if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 3, b, (unsigned)page);
+      active = false;
+    }
+  }
+  const int inside = start & ((1 << p.c.page_shift) - 1);
+  const size_t page_head = active ? (size_t)page * p.c.kv_heads + head : 0;
+  const __half* src = (is_v ? p.v : p.k) + (p.e.q_offsets ? (long long)row0 * p.token_stride : (long long)b * p.batch_stride) +
+                      (long long)head * p.head_stride;
+  uint8_t* codes = (is_v ? p.c.v : p.c.k) + ((page_head << p.c.page_shift) + inside) * D;
+  float* scale = (is_v ? p.c.vs : p.c.ks) + (page_head << (p.c.page_shift - p.c.block_shift)) + (inside >> p.c.block_shift);
+  const int held = pos0 - start;      // tokens that the block held before, where positive
+  const int end = pos0 + n - start;   // rows [max(held, 0), end) are new
+  const bool goes_on = active && held > 0;
+  const float s_old = goes_on ? *scale : 0.0f;
+
+  uint4 x[U];
+  uint32_t mx = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * p.unit + t, r = i / kPieces, piece = i % kPieces;
+    x[u] = make_uint4(0, 0, 0, 0);
+    if (active && r >= held && r < end && r < (1 << p.c.block_shift))
+      x[u] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)(start + r - pos0) * p.token_stride + piece * 8));
+    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu), __vmaxu2(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu)));
+  }
+  mx = __reduce_max_sync(0xffffffffu, max(mx & 0xffffu, mx >> 16));
+  if (p.unit > 32) {  // the same for the whole grid
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) s_max[warp] = mx;
+    __syncthreads();
+    const int w0 = warp & ~(p.unit / 32 - 1);
+    for (int i = 0; i < p.unit / 32; ++i) mx = max(mx, s_max[w0 + i]);
+  }
+  if (!active) return;
+  const float amax = __half2float(__ushort_as_half((unsigned short)mx));
+  const float now = amax * (1.0f / (TYPE == LIGER_KV8_INT8 ? 127.0f : 448.0f));
+  const float s = goes_on && !(now > s_old) && now == now ? s_old : now;  // a scale that is NaN stays
+  const bool finite = s > 0.0f && s <= 3.0e38f;
+  const float back = finite ? 1.0f / s : 0.0f;
+  if (goes_on && !(s == s_old)) {
+    const float ratio = s_old * back;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = u * p.unit + t, r = i / kPieces, piece = i % kPieces;
+      if (r < held && r < (1 << p.c.block_shift)) {
+        uint2* at = reinterpret_cast<uint2*>(codes + (size_t)r * D + piece * 8);
+        uint2 c = make_uint2(0, 0);
+        if (finite) {
+          c = *at;
+          float f[4];
+          kv8_decode4<TYPE>(c.x, f);
+          c.x = kv8_encode4<TYPE>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+          kv8_decode4<TYPE>(c.y, f);
+          c.y = kv8_encode4<TYPE>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+        }
+        *at = c;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * p.unit + t, r = i / kPieces, piece = i % kPieces;
+    if (r >= held && r < end && r < (1 << p.c.block_shift)) {
+      uint2 c = make_uint2(0, 0);
+      if (finite) {
+        float f[8];
+        unpack8(x[u], f);
+        c.x = kv8_encode4<TYPE>(f[0] * back, f[1] * back, f[2] * back, f[3] * back);
+        c.y = kv8_encode4<TYPE>(f[4] * back, f[5] * back, f[6] * back, f[7] * back);
+      }
+      *reinterpret_cast<uint2*>(codes + (size_t)r * D + piece * 8) = c;
+    }
+  }
+  if (t == 0) *scale = s;
+}
+
+template <int D, int U>
+int launch_append(const AppendParams& p, int type, cudaStream_t stream) {
+  const long long units = 2ll * p.c.kv_heads * p.blocks, per = kAppendThreads / p.unit;
+  const dim3 grid((unsigned)((units + per - 1) / per), p.e.batch);
+  if (type == LIGER_KV8_INT8)
+    kv8_append_kernel<D, LIGER_KV8_INT8, U><<<grid, kAppendThreads, 0, stream>>>(p);
+  else
+    kv8_append_kernel<D, LIGER_KV8_E4M3, U><<<grid, kAppendThreads, 0, stream>>>(p);
+  return check_launch("kv8_append_kernel");
+}
+
+}  // namespace
+}  // namespace liger
+
+using namespace liger;
+
+extern "C" int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_append_args* a, void* stream) {
+  if (!a) return set_error(LIGER_ERR_INVALID, "kv8_append: args is NULL");
+  int rc = kv8_check("kv8_append", cache, a->layer);
+  if (rc != LIGER_OK) return rc;
+  if (a->layer < 0) return set_error(LIGER_ERR_INVALID, "kv8_append: layer %d", a->layer);
+  if (!a->k || !a->v || !a->positions) return set_error(LIGER_ERR_INVALID, "kv8_append: a pointer is NULL");
+  if (((uintptr_t)a->k | (uintptr_t)a->v) & 15u) return set_error(LIGER_ERR_INVALID, "kv8_append: k / v must be 16-byte aligned");
+  if (((uintptr_t)a->positions | (uintptr_t)a->slots) & 3u)
+    return set_error(LIGER_ERR_INVALID, "kv8_append: positions and slots must be 4-byte aligned");
+  rc = kv8_check_tokens("kv8_append", a->q_offsets, a->batch, a->q_len, a->total_tokens, a->batch_stride, a->token_stride, a->head_stride);
+  if (rc != LIGER_OK) return rc;
+  const DeviceInfo* dev = current_device();
+  if (!dev) return LIGER_ERR_CUDA;
+  AppendParams p{};
+  p.c = kv8_layer(cache, a->layer);
+  p.e = Kv8Entries{a->q_offsets, a->slots, a->batch, a->q_len, a->total_tokens};
+  p.k = (const __half*)a->k;
+  p.v = (const __half*)a->v;
+  p.positions = a->positions;
+  p.batch_stride = a->batch_stride;
+  p.token_stride = a->token_stride;
+  p.head_stride = a->head_stride;
+  p.status = dev->status_dev;
+  // q_len tokens that begin at the last place of a block touch this many
+  p.blocks = (int)(((long long)a->q_len + cache->scale_block - 2) / cache->scale_block) + 1;
+  const int pieces = cache->scale_block * (cache->head_dim / 8);
+  p.unit = pieces / 8 < 32 ? 32 : pieces / 8;
+  if (2ll * p.c.kv_heads * p.blocks > 0x7fffffffll * (kAppendThreads / p.unit))
+    return set_error(LIGER_ERR_UNSUPPORTED, "kv8_append: q_len %d x kv_heads %d is too large", a->q_len, cache->kv_heads);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (cache->head_dim == 128) return launch_append<128, 8>(p, cache->type, s);
+  return pieces / 8 < 32 ? launch_append<64, 4>(p, cache->type, s) : launch_append<64, 8>(p, cache->type, s);
+}

@@ -1,0 +1,692 @@
+// Attention over the paged 8-bit cache for few query rows per key head (a decode step, a few drafted tokens).
+//
+// Bound by HBM: every code of the cache is read once and used for all query rows of its key head.  What has to be done per code
+// is kept small enough to hide under that: a code becomes an fp16 number (exactly) with one or two instructions and goes
+// into mma.sync, 16 keys x 8 query rows at a time.
+//
+//   S^T[key, row] = K Q^T    A = 16 keys x 16 dims, B = 16 dims x 8 rows.  Which dims stand at which k of a product does not
+//                            matter as long as A and B agree, so a lane takes 16 contiguous bytes of a key at a time.
+//   O^T[dim, row] += V^T P^T A = 16 dims x 16 keys: a lane holds 16 contiguous dims of four keys and pairs the keys' bytes.
+//                            P^T comes out of the S^T accumulators by an 8x8 transpose (movmatrix).
+//
+// Rows are (new token, head of the group) pairs, 8 * NT of them a tile.  Scales: S is multiplied by its key block's scale in
+// fp32.  The value scale goes into P: w = p * (scale / reference), where the reference follows the scales in powers of
+// 16 (the accumulators are rescaled when it moves), so that w stays where fp16 is precise.  P is split into a leading and a
+// trailing fp16 part, two products, so that its rounding does not show in the result; there is tensor throughput to spare here.  The running
+// maximum is moved only when some score exceeds it by 2^8, which a warp finds with one vote.
+//
+// Work is counted in steps of 16 keys of one (sequence, key head, row tile), all sequences' steps in one line, and every CTA
+// takes an equal share of the line whatever the lengths are; where a share begins or ends inside a tile the partial (maximum,
+// sum, accumulator) goes to scratch and a second, small kernel joins the parts.  When max_kv_len is small, a CTA takes a whole
+// tile and nothing is left to join.  Inside a CTA the four warps take every fourth step of a segment, each with its own
+// ring of stages in shared memory that it fills with 16-byte asynchronous copies.
+#include "kv8.cuh"
+
+namespace liger {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStep = 16;            // keys of a step
+constexpr int kMinSteps = 16;        // steps that are worth a CTA
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnParams {
+  Kv8Layer c;
+  Kv8Entries e;
+  const __half* q;
+  __half* out;
+  const int* kv_lens;
+  long long q_batch_stride, q_token_stride, q_head_stride;
+  int heads, group, max_kv_len, ldo, causal;
+  float scale_log2;
+  int whole_tiles;   // 1: CTA = tile (grid: tiles of an entry, entries); 0: equal shares of the line
+  int tiles;         // most tiles of an entry
+  float* parts;      // [2 * CTAs] partial results
+  DeviceStatus* status;
+};
+
+template <int D, int NT>
+struct Cfg {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kStage = 2 * kStep * D;                       // K and V of a step
+  static constexpr int kStages = D == 128 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 12 : 8);
+  static constexpr int kMerge = kWarps * kRows * (D + 4) * 4;        // accumulators of the warps
+  static constexpr int kSmem = kWarps * kStages * kStage + kMerge;
+  static constexpr int kPart = kRows * (D + 2);                      // floats of a partial result: maxima, sums, accumulators
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// An entry of the call with everything checked: n new tokens (rows row0 ..), len keys.  A bad length or slot gives len 0.
+struct Entry {
+  int n, row0, len, slot;
+};
+__device__ __forceinline__ Entry load_entry(const AttnParams& p, int b, bool report) {
+  Entry e;
+  if (!kv8_rows(p.e, b, e.n, e.row0) && report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention, b, 0);
+  e.len = __ldg(p.kv_lens + b);
+  e.slot = kv8_slot(p.e, b);
+  if (e.len < 0 || e.len > p.max_kv_len || e.slot < 0 || e.slot >= p.c.slots || e.len > ((long long)p.c.max_pages << p.c.page_shift)) {
+    if (report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 1, b, (unsigned)e.len);
+    e.len = 0;
+  }
+  return e;
+}
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const AttnParams& p, const Entry& e) { return (e.n * p.group + ROWS - 1) / ROWS; }
+// an entry without keys still has rows to fill with zeros
+__device__ __forceinline__ int steps_of(const Entry& e) { return max(1, (e.len + kStep - 1) / kStep); }
+template <int ROWS>
+__device__ __forceinline__ long long line_of(const AttnParams& p, const Entry& e) {
+  return (long long)p.c.kv_heads * row_tiles<ROWS>(p, e) * steps_of(e);
+}
+
+__device__ __forceinline__ int ctas_used(long long total, int ctas) {
+  const long long want = (total + kMinSteps - 1) / kMinSteps;
+  return (int)(want < ctas ? want : ctas);
+}
+__device__ __forceinline__ long long share_begin(long long total, int used, int cta) { return total * cta / used; }
+__device__ __forceinline__ int share_of(long long total, int used, long long at) {  // the CTA whose share has step `at`
+  int c = (int)(at * used / total);
+  while (share_begin(total, used, c + 1) <= at) ++c;
+  while (share_begin(total, used, c) > at) --c;
+  return c;
+}
+
+// Sum over the entries, and the entry that has place `at` of the line (at = f(total)); all threads of the CTA get the answer.
+template <int ROWS, int THREADS, typename F>
+__device__ __forceinline__ void find_place(const AttnParams& p, F place, long long& total, long long& at, int& b_out, long long& b_first) {
+  __shared__ long long s_warp[THREADS / 32], s_first;
+  __shared__ int s_b;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long mine = 0;
+  for (int b = threadIdx.x; b < p.e.batch; b += THREADS) mine += line_of<ROWS>(p, load_entry(p, b, false));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) s_warp[warp] = mine;
+  if (threadIdx.x == 0) s_b = -1;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) total += s_warp[w];
+  at = place(total);
+  __syncthreads();
+  if (at < 0 || at >= total) { b_out = -1; return; }  // the same in all threads
+  long long before = 0;
+  for (int base = 0; base < p.e.batch; base += THREADS) {
+    const int b = base + threadIdx.x;
+    const long long v = b < p.e.batch ? line_of<ROWS>(p, load_entry(p, b, false)) : 0;
+    long long incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    long long all = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) incl += s_warp[w];
+      all += s_warp[w];
+    }
+    if (at >= before + incl - v && at < before + incl) { s_b = b; s_first = before + incl - v; }
+    before += all;
+    __syncthreads();
+    if (s_b >= 0) break;
+  }
+  b_out = s_b;
+  b_first = s_first;
+}
+
+// 16-byte chunk `c` of key `r` of a step.  The xor spreads both ways of reading over all banks: a lane quad reads a key
+// across (K), and eight lanes with one dim range each read four keys (V).
+template <int D>
+__device__ __forceinline__ int stage_at(int r, int c) {
+  if (D == 128) return r * 128 + ((c ^ ((r & 6) ^ ((r & 1) << 2))) << 4);
+  return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (r & 6)) << 4);  // two keys a line
+}
+
+template <int D, int TYPE, int NT>
+__global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnParams p) {
+  using C = Cfg<D, NT>;
+  constexpr int kKk = D / 16;             // k-steps of a score product = dim tiles of an output product
+  extern __shared__ __align__(128) uint8_t smem_kv8[];
+  __shared__ float s_m[kWarps][C::kRows], s_l[kWarps][C::kRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem_kv8 + warp * C::kStages * C::kStage;
+  const uint32_t ring_u = smem_u32(ring);
+  float* merge = reinterpret_cast<float*>(smem_kv8 + kWarps * C::kStages * C::kStage);
+
+  // this CTA's share: places [at, end) of the line, beginning in entry b whose places start at b_first
+  long long total = 0, at = 0, end = 0, b_first = 0;
+  int b, used = 0;
+  const int cta = blockIdx.x;
+  Entry e;
+  if (p.whole_tiles) {
+    b = blockIdx.y;
+    e = load_entry(p, b, blockIdx.x == 0 && threadIdx.x == 0);
+    const int tile = blockIdx.x;
+    if (tile >= p.c.kv_heads * row_tiles<C::kRows>(p, e)) return;
+    at = (long long)tile * steps_of(e);
+    end = at + steps_of(e);
+  } else {
+    if (cta == 0)
+      for (int i = threadIdx.x; i < p.e.batch; i += kThreads) load_entry(p, i, true);
+    find_place<C::kRows, kThreads>(
+        p, [&](long long all) {
+          used = ctas_used(all, gridDim.x);
+          return cta < used ? share_begin(all, used, cta) : -1;
+        },
+        total, at, b, b_first);
+    if (b < 0) return;
+    end = share_begin(total, used, cta + 1);
+    e = load_entry(p, b, false);
+  }
+  const long long share0 = at;
+
+  while (at < end) {
+    const int steps = steps_of(e);
+    const long long inside = at - b_first;
+    const int tile = (int)(inside / steps), s_begin = (int)(inside % steps);
+    const int tiles = row_tiles<C::kRows>(p, e);
+    const int head = tile / tiles, row_base = (tile % tiles) * C::kRows;
+    const int s_end = (int)((long long)steps < s_begin + (end - at) ? steps : s_begin + (end - at));
+    const int rows = e.n * p.group;
+
+    // this lane's rows: as B operand row g of each n-tile, as accumulator column 2t, 2t + 1
+    uint32_t qf[NT][kKk][2];
+    int limit[NT][2], limit_min = e.len;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row_base + nt * 8 + g;
+      uint4 x[D / 32];
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) x[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int token = r / p.group;
+        const __half* src = p.q + (p.e.q_offsets ? (long long)(e.row0 + token) * p.q_token_stride
+                                                 : (long long)b * p.q_batch_stride + (long long)token * p.q_token_stride) +
+                            (long long)(head * p.group + r % p.group) * p.q_head_stride;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          x[2 * h] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16));
+          x[2 * h + 1] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16 + 8));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        qf[nt][2 * i][0] = x[i].x; qf[nt][2 * i][1] = x[i].y;
+        qf[nt][2 * i + 1][0] = x[i].z; qf[nt][2 * i + 1][1] = x[i].w;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int rc = row_base + nt * 8 + 2 * t + c;
+        limit[nt][c] = rc >= rows ? 0 : p.causal ? min(e.len, max(0, e.len - e.n + rc / p.group + 1)) : e.len;
+      }
+    }
+    if (p.causal) limit_min = min(e.len, max(0, e.len - e.n + row_base / p.group + 1));
+
+    float m_ref[NT][2], l_run[NT][2], v_ref = 0.0f;
+    float o[NT][kKk][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
+      l_run[nt][0] = l_run[nt][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kKk; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f; }
+    }
+
+    // this warp's steps: s_begin + warp + i * kWarps, i < count (an entry without keys has none)
+    const int count = e.len > 0 && s_begin + warp < s_end ? (s_end - s_begin - warp + kWarps - 1) / kWarps : 0;
+    const int* row_table = p.c.table + (size_t)e.slot * p.c.max_pages;
+    const int page_mask = (1 << p.c.page_shift) - 1;
+    // page and scales of 32 steps, one per lane: `now` for steps being copied, the lookups of the next 32 under way
+    auto lookup = [&](int i0, int& page, float& ks, float& vs) {
+      const int i = i0 + lane;
+      page = -1;
+      ks = vs = 0.0f;
+      if (i < count) {
+        const int key = (s_begin + warp + i * kWarps) * kStep;
+        page = __ldg(row_table + (key >> p.c.page_shift));
+        if (page < 0 || page >= p.c.num_pages) {
+          report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 2, b, (unsigned)page);
+          page = -1;
+        } else {
+          const size_t ph = (size_t)page * p.c.kv_heads + head;
+          const size_t blk = (ph << (p.c.page_shift - p.c.block_shift)) + ((key & page_mask) >> p.c.block_shift);
+          ks = __ldg(p.c.ks + blk);
+          vs = __ldg(p.c.vs + blk);
+          if (!(vs < INFINITY)) vs = NAN;
+        }
+      }
+    };
+    int page_even, page_odd;  // of windows of 32 steps, by the window's parity: the one in use and the next
+    float ks_even, ks_odd, vs_even, vs_odd;
+    lookup(0, page_even, ks_even, vs_even);
+    lookup(32, page_odd, ks_odd, vs_odd);
+
+    auto copy_step = [&](int i) {
+      if (i < count) {
+        const int page = __shfl_sync(0xffffffffu, (i >> 5) & 1 ? page_odd : page_even, i & 31);
+        if (page >= 0) {
+          const int key = (s_begin + warp + i * kWarps) * kStep;
+          const size_t src = ((((size_t)page * p.c.kv_heads + head) << p.c.page_shift) + (key & page_mask)) * D;
+          const uint32_t dst = ring_u + (i % C::kStages) * C::kStage;
+          constexpr int kChunks = D / 16;
+#pragma unroll
+          for (int j = 0; j < kStep * D / 512; ++j) {
+            const int r = lane / kChunks + j * (32 / kChunks), c = lane % kChunks;
+            const int off = stage_at<D>(r, c);
+            cp_async16(dst + off, p.c.k + src + r * D + c * 16);
+            cp_async16(dst + kStep * D + off, p.c.v + src + r * D + c * 16);
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int i = 0; i < C::kStages - 1; ++i) copy_step(i);
+
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      // window boundary: steps up to i + kStages - 2 are under way; once the copies reach window w + 1, window w - 1 is done with
+      if ((i & 31) == 0 && i > 0) {
+        if ((i >> 5) & 1) lookup(i + 32, page_even, ks_even, vs_even);
+        else lookup(i + 32, page_odd, ks_odd, vs_odd);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
+      __syncwarp();
+      const int odd = (i >> 5) & 1;
+      const int page = __shfl_sync(0xffffffffu, odd ? page_odd : page_even, i & 31);
+      const float ks = __shfl_sync(0xffffffffu, odd ? ks_odd : ks_even, i & 31);
+      const float vs = __shfl_sync(0xffffffffu, odd ? vs_odd : vs_even, i & 31);
+      const int key0 = (s_begin + warp + i * kWarps) * kStep;
+      const uint8_t* sk = ring + (i % C::kStages) * C::kStage;
+      uint8_t* sv = ring + (i % C::kStages) * C::kStage + kStep * D;
+      if (page >= 0) {
+        if (key0 + kStep > e.len) {  // behind the last key lies anything: it must not meet a weight of 0 as a NaN
+          constexpr int kChunks = D / 16;
+          for (int j = lane; j < kStep * kChunks; j += 32)
+            if (key0 + j / kChunks >= e.len) *reinterpret_cast<uint4*>(sv + stage_at<D>(j / kChunks, j % kChunks)) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
+        // S^T = K Q^T
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          const uint4 ka = *reinterpret_cast<const uint4*>(sk + stage_at<D>(g, t + 4 * h));
+          const uint4 kb = *reinterpret_cast<const uint4*>(sk + stage_at<D>(g + 8, t + 4 * h));
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a = kv8_bias<TYPE>(wa[w]), c = kv8_bias<TYPE>(wb[w]);
+            const uint32_t a0 = kv8_pair<TYPE, 0>(a), a2 = kv8_pair<TYPE, 1>(a), a1 = kv8_pair<TYPE, 0>(c), a3 = kv8_pair<TYPE, 1>(c);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qf[nt][4 * h + w][0], qf[nt][4 * h + w][1]);
+          }
+        }
+        // scores in units of log2; s[.][0], [1]: key g, rows 2t, 2t + 1; s[.][2], [3]: key g + 8
+        const float xs = ks * p.scale_log2;
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[nt][c] *= xs;
+          if (key0 + kStep > limit_min) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (key0 + g + (c >> 1) * 8 >= limit[nt][c & 1]) s[nt][c] = -INFINITY;
+          }
+          grow |= fmaxf(s[nt][0], s[nt][2]) > m_ref[nt][0] + 8.0f || fmaxf(s[nt][1], s[nt][3]) > m_ref[nt][1] + 8.0f;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              if (mx > m_ref[nt][c]) {
+                const float alpha = exp2_approx(m_ref[nt][c] - mx);  // 0 the first time
+                m_ref[nt][c] = mx;
+                l_run[nt][c] *= alpha;
+#pragma unroll
+                for (int d = 0; d < kKk; ++d) { o[nt][d][c] *= alpha; o[nt][d][c + 2] *= alpha; }
+              }
+            }
+          }
+        }
+        // weights.  The value scale relative to the reference; the reference moves by powers of 16
+        float rel = vs / v_ref;
+        if (!(rel <= 16.0f && rel >= 0.0625f) && vs > 0.0f) {
+          const float back = v_ref / vs;  // 0 the first time
+          v_ref = vs;
+          rel = 1.0f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int d = 0; d < kKk; ++d) { o[nt][d][0] *= back; o[nt][d][1] *= back; o[nt][d][2] *= back; o[nt][d][3] *= back; }
+        }
+        if (vs == 0.0f) rel = 0.0f;
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float m = m_ref[nt][c & 1];
+            const float pr = exp2_approx(s[nt][c] - (m == -INFINITY ? 0.0f : m));
+            l_run[nt][c & 1] += pr;
+            w[c] = s[nt][c] == -INFINITY ? 0.0f : pr * rel;  // a key that is not seen has no weight, whatever its scale is
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const __half2 hi = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+            const float2 back = __half22float2(hi);
+            ph[nt][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+            pl[nt][i] = transpose8x8(pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
+          }
+        }
+        // O^T += V^T P^T
+        constexpr int kWords = D / 32;  // 4-byte words of dims that a lane holds of each key
+        uint32_t vw[4][kWords];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = 2 * t + (j & 1) + (j >> 1) * 8;
+          if (D == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(sv + stage_at<D>(key, g));
+            vw[j][0] = x.x; vw[j][1] = x.y; vw[j][2 % kWords] = x.z; vw[j][3 % kWords] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(sv + stage_at<D>(key, g >> 1) + (g & 1) * 8);
+            vw[j][0] = x.x; vw[j][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          const uint32_t x0 = kv8_bias<TYPE>(vw[0][w]), x1 = kv8_bias<TYPE>(vw[1][w]), x2 = kv8_bias<TYPE>(vw[2][w]), x3 = kv8_bias<TYPE>(vw[3][w]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t ab = __byte_perm(x0, x1, half ? 0x7362 : 0x5140), cd = __byte_perm(x2, x3, half ? 0x7362 : 0x5140);
+            const uint32_t a0 = kv8_pair<TYPE, 0>(ab), a1 = kv8_pair<TYPE, 1>(ab), a2 = kv8_pair<TYPE, 0>(cd), a3 = kv8_pair<TYPE, 1>(cd);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+              mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // all lanes have read stage i before it is filled again
+      copy_step(i + C::kStages - 1);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // join the warps
+    float m_w[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float l = l_run[nt][c];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        m_w[nt][c] = m_ref[nt][c];
+        const int r = nt * 8 + 2 * t + c;
+        if (g == 0) { s_m[warp][r] = m_w[nt][c]; s_l[warp][r] = l; }
+        float* dst = merge + (warp * C::kRows + r) * (D + 4) + g * (D / 8);
+#pragma unroll
+        for (int d = 0; d < kKk; d += 2)
+          *reinterpret_cast<float4*>(dst + 2 * d) = make_float4(o[nt][d][c] * v_ref, o[nt][d][c + 2] * v_ref, o[nt][d + 1][c] * v_ref, o[nt][d + 1][c + 2] * v_ref);
+      }
+    }
+    __syncthreads();
+    const bool complete = s_begin == 0 && s_end == steps;
+    float* part = p.parts + (size_t)(2 * cta + (at == share0 && s_begin > 0 ? 0 : 1)) * C::kPart;
+    for (int i = threadIdx.x; i < C::kRows * D / 4; i += kThreads) {
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+      if (row_base + r >= rows) continue;
+      float m = s_m[0][r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][r]);
+      float l = 0.0f;
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float lw = s_l[w][r];
+        const float f = lw == 0.0f ? 0.0f : lw == lw ? exp2_approx(s_m[w][r] - m) : 1.0f;  // saw nothing / a NaN stays
+        const float4 x = *reinterpret_cast<const float4*>(merge + (w * C::kRows + r) * (D + 4) + d);
+        l += f * lw;
+        a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+      }
+      if (complete) {
+        const int token = (row_base + r) / p.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        __half* dst = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + (row_base + r) % p.group) * D + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(a.x * inv, a.y * inv), pack_half2(a.z * inv, a.w * inv));
+      } else {
+        if (d == 0) { part[r] = m; part[C::kRows + r] = l; }
+        *reinterpret_cast<float4*>(part + 2 * C::kRows + r * D + d) = a;
+      }
+    }
+    __syncthreads();
+
+    at += s_end - s_begin;
+    if (at < end && at == b_first + (long long)p.c.kv_heads * tiles * steps) {
+      b_first = at;
+      do {
+        ++b;
+        e = load_entry(p, b, false);
+      } while (e.n == 0);  // entries without new tokens have no place in the line
+    }
+  }
+}
+
+constexpr int kJoinThreads = 256;
+
+// Joins the parts of the tiles that more than one CTA worked on.  CTA (c, r) has row r of the tile that lies across the border
+// between shares c and c + 1, where that is the tile's first border.
+template <int D, int NT>
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const AttnParams p, int ctas) {
+  using C = Cfg<D, NT>;
+  constexpr int kW = kJoinThreads / 32;
+  __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
+  const int border = blockIdx.x + 1, r = blockIdx.y;
+  long long total, at, b_first;
+  int b, used = 0;
+  find_place<C::kRows, kJoinThreads>(
+      p, [&](long long all) {
+        used = ctas_used(all, ctas);
+        return border < used ? share_begin(all, used, border) : -1;
+      },
+      total, at, b, b_first);
+  if (b < 0) return;
+  const Entry e = load_entry(p, b, false);
+  const int steps = steps_of(e), tiles = row_tiles<C::kRows>(p, e);
+  const int tile = (int)((at - b_first) / steps);
+  const long long t0 = b_first + (long long)tile * steps, t1 = t0 + steps;
+  if (t0 == at || share_begin(total, used, border - 1) > t0) return;  // nothing across this border, or not the first border
+  const int c0 = border - 1, c1 = share_of(total, used, t1 - 1);
+  const int head = tile / tiles, row = (tile % tiles) * C::kRows + r;
+  if (row >= e.n * p.group) return;
+  // shares c0 .. c1; the first one began the tile (unless its share began with it, that is its second slot)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.0f, a[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) a[i] = 0.0f;
+  for (int c = c0 + warp; c <= c1; c += kW) {
+    const float* part = p.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * C::kPart;
+    const float pm = part[r], pl = part[C::kRows + r];
+    float x[D / 32];
+    if (D == 128) {
+      const float4 v = *reinterpret_cast<const float4*>(part + 2 * C::kRows + r * D + lane * 4);
+      x[0] = v.x; x[1] = v.y; x[2 % (D / 32)] = v.z; x[3 % (D / 32)] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(part + 2 * C::kRows + r * D + lane * 2);
+      x[0] = v.x; x[1] = v.y;
+    }
+    if (pl == 0.0f) continue;  // saw nothing
+    const float m_new = fmaxf(m, pm);
+    const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - m_new), fb = exp2_approx(pm - m_new);
+    m = m_new;
+    l = l * fa + pl * fb;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) a[i] = a[i] * fa + x[i] * fb;
+  }
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) s_a[warp][lane * (D / 32) + i] = a[i];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float mm = s_m[0];
+    for (int w = 1; w < kW; ++w) mm = fmaxf(mm, s_m[w]);
+    float ll = 0.0f, y = 0.0f;
+    for (int w = 0; w < kW; ++w) {
+      if (s_l[w] == 0.0f) continue;
+      const float f = exp2_approx(s_m[w] - mm);
+      ll += f * s_l[w];
+      y += f * s_a[w][threadIdx.x];
+    }
+    const int token = row / p.group;
+    p.out[(size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D + threadIdx.x] =
+        __float2half_rn(ll == 0.0f ? 0.0f : y / ll);
+  }
+}
+
+struct Plan {
+  int nt, rows, tiles, whole_tiles, ctas;
+  size_t part_floats;
+};
+
+// How a call is launched; a function of its sizes alone.
+Plan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm_count) {
+  Plan p;
+  const long long rows = (long long)a->q_len * (a->heads / c->kv_heads);
+  p.nt = rows > 8 ? 2 : 1;
+  p.rows = 8 * p.nt;
+  const long long tiles = (long long)c->kv_heads * ((rows + p.rows - 1) / p.rows);
+  p.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
+  p.whole_tiles = a->max_kv_len <= 512;
+  p.ctas = 2 * sm_count;
+  p.part_floats = p.whole_tiles ? 0 : (size_t)2 * p.ctas * p.rows * (c->head_dim + 2);
+  return p;
+}
+
+template <int D, int TYPE, int NT>
+int launch(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
+  using C = Cfg<D, NT>;
+  LIGER_CUDA_TRY(cudaFuncSetAttribute(kv8_attention_kernel<D, TYPE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  const dim3 grid = pl.whole_tiles ? dim3(pl.tiles, ap.e.batch) : dim3(pl.ctas);
+  kv8_attention_kernel<D, TYPE, NT><<<grid, kThreads, C::kSmem, s>>>(ap);
+  int rc = check_launch("kv8_attention_kernel");
+  if (rc != LIGER_OK || pl.whole_tiles) return rc;
+  kv8_attention_join_kernel<D, NT><<<dim3(pl.ctas - 1, pl.rows), kJoinThreads, 0, s>>>(ap, pl.ctas);
+  return check_launch("kv8_attention_join_kernel");
+}
+
+template <int D, int TYPE>
+int launch_rows(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
+  return pl.nt == 1 ? launch<D, TYPE, 1>(ap, pl, s) : launch<D, TYPE, 2>(ap, pl, s);
+}
+
+int check_args(const liger_kv8_cache* c, const liger_kv8_attention_args* a) {
+  if (!a) return set_error(LIGER_ERR_INVALID, "kv8_attention: args is NULL");
+  int rc = kv8_check("kv8_attention", c, a->layer);
+  if (rc != LIGER_OK) return rc;
+  if (a->layer < 0) return set_error(LIGER_ERR_INVALID, "kv8_attention: layer %d", a->layer);
+  if (a->heads <= 0 || a->heads % c->kv_heads)
+    return set_error(LIGER_ERR_INVALID, "kv8_attention: heads = %d must be a positive multiple of kv_heads = %d", a->heads, c->kv_heads);
+  rc = kv8_check_tokens("kv8_attention", a->q_offsets, a->batch, a->q_len, a->total_tokens, a->q_batch_stride, a->q_token_stride,
+                        a->q_head_stride);
+  if (rc != LIGER_OK) return rc;
+  if ((long long)a->q_len * (a->heads / c->kv_heads) > (1 << 30))
+    return set_error(LIGER_ERR_UNSUPPORTED, "kv8_attention: q_len * heads / kv_heads <= 2^30");
+  if (a->max_kv_len < 0) return set_error(LIGER_ERR_INVALID, "kv8_attention: max_kv_len must not be negative");
+  if (a->ldo % 8 || a->ldo < (long long)a->heads * c->head_dim)
+    return set_error(LIGER_ERR_INVALID, "kv8_attention: ldo = %d must be a multiple of 8 and >= heads * head_dim = %lld", a->ldo,
+                     (long long)a->heads * c->head_dim);
+  return LIGER_OK;
+}
+
+// the SM count that workspaces are sized for where no device can be asked
+constexpr int kAssumedSms = 148;
+
+}  // namespace
+}  // namespace liger
+
+using namespace liger;
+
+extern "C" size_t liger_kv8_attention_scratch_bytes(const liger_kv8_cache* cache, const liger_kv8_attention_args* args) {
+  if (check_args(cache, args) != LIGER_OK) return 0;
+  int dev = -1, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    sms = kAssumedSms;
+  }
+  return plan_of(cache, args, sms).part_floats * sizeof(float);
+}
+
+extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8_attention_args* a, void* stream) {
+  int rc = check_args(cache, a);
+  if (rc != LIGER_OK) return rc;
+  if (!a->q || !a->out || !a->kv_lens) return set_error(LIGER_ERR_INVALID, "kv8_attention: a pointer is NULL");
+  if (((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->scratch) & 15u)
+    return set_error(LIGER_ERR_INVALID, "kv8_attention: q, out and scratch must be 16-byte aligned");
+  if (((uintptr_t)a->kv_lens | (uintptr_t)a->slots) & 3u)
+    return set_error(LIGER_ERR_INVALID, "kv8_attention: kv_lens and slots must be 4-byte aligned");
+  if (!a->scratch && plan_of(cache, a, kAssumedSms).part_floats) return set_error(LIGER_ERR_INVALID, "kv8_attention: scratch is NULL");
+  const DeviceInfo* dev = current_device();
+  if (!dev) return LIGER_ERR_CUDA;
+  const Plan pl = plan_of(cache, a, dev->sm_count);
+  const size_t need = pl.part_floats * sizeof(float);
+  if (a->scratch_bytes < need)
+    return set_error(LIGER_ERR_TOO_LARGE, "kv8_attention: scratch has %zu bytes, %zu are needed", a->scratch_bytes, need);
+  if (pl.tiles == 0x7fffffff) return set_error(LIGER_ERR_UNSUPPORTED, "kv8_attention: q_len %d x heads %d is too large", a->q_len, a->heads);
+  AttnParams p{};
+  p.c = kv8_layer(cache, a->layer);
+  p.e = Kv8Entries{a->q_offsets, a->slots, a->batch, a->q_len, a->total_tokens};
+  p.q = (const __half*)a->q;
+  p.out = (__half*)a->out;
+  p.kv_lens = a->kv_lens;
+  p.q_batch_stride = a->q_batch_stride;
+  p.q_token_stride = a->q_token_stride;
+  p.q_head_stride = a->q_head_stride;
+  p.heads = a->heads;
+  p.group = a->heads / cache->kv_heads;
+  p.max_kv_len = a->max_kv_len;
+  p.ldo = a->ldo;
+  p.causal = a->causal;
+  p.scale_log2 = a->scale * kLog2e;
+  p.whole_tiles = pl.whole_tiles;
+  p.tiles = pl.tiles;
+  p.parts = (float*)a->scratch;
+  p.status = dev->status_dev;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (cache->head_dim == 128)
+    return cache->type == LIGER_KV8_INT8 ? launch_rows<128, LIGER_KV8_INT8>(p, pl, s) : launch_rows<128, LIGER_KV8_E4M3>(p, pl, s);
+  return cache->type == LIGER_KV8_INT8 ? launch_rows<64, LIGER_KV8_INT8>(p, pl, s) : launch_rows<64, LIGER_KV8_E4M3>(p, pl, s);
+}

@@ -38,6 +38,7 @@ extern "C" {
 
 /* bits of the sticky device status word */
 #define LIGER_DEV_TIMEOUT 1u /* a bounded device-side wait ran out */
+#define LIGER_DEV_BAD_INDEX 2u /* data on the device named a page, slot, position or row that does not exist; it was left out */
 
 /* Message describing the last error returned to the calling thread ("" if none). */
 LIGER_API const char* liger_last_error(void);
@@ -215,6 +216,129 @@ LIGER_API size_t liger_attention_decode_noalloc_max_bytes(void);
 LIGER_API int liger_attention_decode_noalloc(const void* q, const void* k_cache, const void* v_cache, void* out, int batch,
                                              int heads, int kv_len, int kv_stride, int head_dim, int ldo, float scale,
                                              void* stream);
+
+/* ------------------------------------------------------------------------------------------ */
+/* A paged key/value cache held in 8 bits                                                     */
+/* ------------------------------------------------------------------------------------------ */
+
+/*
+ * The cache keeps keys and values as 8-bit codes with one fp32 scale for each block of `scale_block` tokens and
+ * head: value = code * scale.  Tokens live in pages; a sequence is a row ("slot") of a page table that is shared by
+ * all layers.  It holds half the bytes of the fp16 cache that liger_attention_decode reads, has no common length, and
+ * sequences can share pages.  No reference counterpart: the reference has no KV cache.
+ *
+ * The struct is read on the host during a call; every array lies in device memory of the current device and belongs
+ * to the caller.  Requirements: head_dim 64 or 128; page_size a power of two, 16 .. 256; scale_block a power of two,
+ * 16 .. min(128, page_size); k_pages / v_pages 16-byte aligned.  The layout is [layers][num_pages][kv_heads][page_size]
+ * [head_dim], so that the tokens of one page and head are one contiguous run of bytes.
+ *
+ * What the arrays on the device say (tables, lengths, offsets) is checked by the kernels, not by the host: a page,
+ * slot, position or row that does not exist is left out, and LIGER_DEV_BAD_INDEX is set in the sticky device status.
+ *
+ * A block into which a value that is not finite was written reads as NaN: its scale is then not finite and its codes are 0.
+ */
+#define LIGER_KV8_INT8 0 /* codes -127 .. 127 */
+#define LIGER_KV8_E4M3 1 /* fp8, 4 exponent and 3 fraction bits, largest 448 */
+
+typedef struct liger_kv8_cache {
+  void* k_pages;   /* [layers, num_pages, kv_heads, page_size, head_dim] codes */
+  void* v_pages;
+  float* k_scales; /* [layers, num_pages, kv_heads, page_size / scale_block] */
+  float* v_scales;
+  int* page_table; /* [slots, max_pages]: the pages of a slot in order, -1 behind the last one */
+  int* page_count; /* [slots]: how many pages a slot holds (only for the page operators; else NULL) */
+  int* page_refs;  /* [num_pages]: how many table entries name a page, 0 = free (only for the page operators; else NULL) */
+  int layers, num_pages, kv_heads, page_size, scale_block, head_dim, type;
+  int slots, max_pages;
+} liger_kv8_cache;
+
+/*
+ * Writes new keys and values of `layer` behind the tokens that the slots hold.  Sequence b of the call is slot slots[b]
+ * (slot b when slots is NULL) and its tokens go to positions positions[b], positions[b] + 1, ...  With q_offsets NULL every
+ * sequence brings q_len tokens, token i's head h at k + b * batch_stride + i * token_stride + h * head_stride (elements;
+ * LIGER_EPI_QKV_SPLIT's [B, h, S, D] outputs and [tokens, h * D] rows both fit).  With q_offsets (device, [batch + 1],
+ * non-decreasing) sequence b brings tokens q_offsets[b] .. q_offsets[b+1] - 1 of total_tokens, at most q_len, at
+ * k + token * token_stride + h * head_stride.
+ *
+ * A block's scale is (largest magnitude among its new values) * fp32(1 / largest code); a block that already holds tokens
+ * of the sequence keeps its scale unless the new one is larger, and its codes are then rounded again to the larger scale.
+ * code = round-to-nearest-even(fp32(x * fp32(1 / scale))), saturated.  A block of zeros has scale 0.
+ * The pages have to be there (liger_kv8_reserve) and belong to the slot alone from positions[b] on (liger_kv8_fork sees
+ * to that).  A slot that is named twice in one call is written for its first entry only (LIGER_DEV_BAD_INDEX).
+ * Strides are multiples of 8 elements, k and v 16-byte aligned.
+ */
+typedef struct liger_kv8_append_args {
+  const void* k; /* fp16 */
+  const void* v;
+  const int* q_offsets; /* device [batch + 1] or NULL */
+  const int* slots;     /* device [batch] or NULL */
+  const int* positions; /* device [batch] */
+  long long batch_stride, token_stride, head_stride;
+  int batch, q_len, total_tokens, layer;
+} liger_kv8_append_args;
+
+LIGER_API int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_append_args* args, void* stream);
+
+/*
+ * Attention of new queries over the cache: out = softmax(scale * q K^T) V in fp32, written as fp16.  heads is a multiple of
+ * cache->kv_heads; query head h reads key head h / (heads / kv_heads).  Sequence b has kv_lens[b] tokens in the cache, the
+ * new ones included; its queries are addressed like the new tokens of liger_kv8_append (q_batch_stride, q_token_stride,
+ * q_head_stride; q_offsets, q_len, total_tokens).  With causal != 0 the i-th of n queries sees the keys at positions up to
+ * kv_lens[b] - n + i, else all kv_lens[b].  A query that sees nothing gets zeros.  Row (token) t of the call, head h goes
+ * to out + t * ldo + h * head_dim; rows that belong to no sequence are left as they were.  max_kv_len bounds kv_lens; it
+ * decides how the work is split, and a sequence that is longer counts as empty (LIGER_DEV_BAD_INDEX), like one whose slot
+ * does not exist.  A key on a page that does not exist is left out.
+ *
+ * scratch holds the partial results of sequences that are split over several thread blocks:
+ * liger_kv8_attention_scratch_bytes() bytes (it reads the sizes in *args, not its pointers), 16-byte aligned, not shared
+ * with a call that may run at the same time, captured graphs included.  ldo % 8 == 0, out and q 16-byte aligned, strides
+ * multiples of 8 elements.
+ */
+typedef struct liger_kv8_attention_args {
+  const void* q; /* fp16 */
+  void* out;     /* [tokens, ldo] fp16 */
+  void* scratch;
+  size_t scratch_bytes;
+  const int* q_offsets; /* device [batch + 1] or NULL */
+  const int* slots;     /* device [batch] or NULL */
+  const int* kv_lens;   /* device [batch] */
+  long long q_batch_stride, q_token_stride, q_head_stride;
+  int batch, heads, q_len, total_tokens;
+  int max_kv_len, ldo, layer, causal;
+  float scale;
+} liger_kv8_attention_args;
+
+LIGER_API size_t liger_kv8_attention_scratch_bytes(const liger_kv8_cache* cache, const liger_kv8_attention_args* args);
+LIGER_API int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8_attention_args* args, void* stream);
+
+/*
+ * Keeping the pages.  All state (page_table, page_count, page_refs) is on the device, so a serving loop never waits for
+ * it; calls on one cache have to be ordered, on one stream or by events.  Free pages are taken lowest number first, in the
+ * order of the entries, so that results do not depend on timing.  done (device [n] or NULL) tells for each entry whether
+ * it was carried out (1) or refused (0).  scratch: liger_kv8_pages_scratch_bytes(cache, n) bytes, 16-byte aligned.
+ *
+ *   reserve  gives slot slots[i] the pages for lens[i] tokens in all; pages that it has stay.  Refused when the pool has too
+ *            few free pages for the entries up to i, when lens[i] needs more than max_pages, and for a slot's second entry
+ *   fork     makes the empty slot dst[i] the first lens[i] tokens of slot src[i]: whole pages are shared, a last page that
+ *            is not full is copied, in all layers.  Refused when dst[i] holds pages or is named before, when src[i] has
+ *            fewer than lens[i] tokens' pages, and when the pool is out of pages for the entries up to i
+ *   free     takes the pages of the slots away; a page is free when no slot names it any more.  A slot may be named twice
+ *   copy     copies page src[i] onto page dst[i] in all layers.  Refused when dst[i] is the target of an earlier entry or
+ *            src[i] the target of any other entry.  Tables and counts stay as they are
+ *   compact  moves the pages in use to the numbers 0 .. live - 1: those behind are moved, in order, to the free numbers
+ *            before.  live (device, 1 int) and moved_to (device [num_pages]: a page's new number, -1 for a free one) may be
+ *            NULL.  n = 0 for its scratch
+ */
+LIGER_API size_t liger_kv8_pages_scratch_bytes(const liger_kv8_cache* cache, int n);
+LIGER_API int liger_kv8_reserve(const liger_kv8_cache* cache, const int* slots, const int* lens, int n, int* done,
+                                void* scratch, size_t scratch_bytes, void* stream);
+LIGER_API int liger_kv8_fork(const liger_kv8_cache* cache, const int* src, const int* dst, const int* lens, int n, int* done,
+                             void* scratch, size_t scratch_bytes, void* stream);
+LIGER_API int liger_kv8_free(const liger_kv8_cache* cache, const int* slots, int n, void* stream);
+LIGER_API int liger_kv8_copy(const liger_kv8_cache* cache, const int* src, const int* dst, int n, int* done, void* scratch,
+                             size_t scratch_bytes, void* stream);
+LIGER_API int liger_kv8_compact(const liger_kv8_cache* cache, int* live, int* moved_to, void* scratch, size_t scratch_bytes,
+                                void* stream);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Row-wise operators                                                                         */
