@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libliger_b200.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared",
+    "--threads", "0",  # source files are compiled side by side
 ]
 
 

@@ -15,11 +15,12 @@
 // trailing fp16 part, two products, so that its rounding does not show in the result; there is tensor throughput to spare here.  The running
 // maximum is moved only when some score exceeds it by 2^8, which a warp finds with one vote.
 //
-// Work is counted in steps of 16 keys of one (sequence, key head, row tile), all sequences' steps in one line, and every CTA
-// takes an equal share of the line whatever the lengths are; where a share begins or ends inside a tile the partial (maximum,
-// sum, accumulator) goes to scratch and a second, small kernel joins the parts.  When max_kv_len is small, a CTA takes a whole
-// tile and nothing is left to join.  Inside a CTA the four warps take every fourth step of a segment, each with its own
-// ring of stages in shared memory that it fills with 16-byte asynchronous copies.
+// Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
+// it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
+// are; warps never wait for one another.  Where a share begins or ends inside a tile the partial (maximum, sum, accumulator)
+// goes to scratch and a second, small kernel joins the parts; it is launched early and waits for the first.  Short calls with few
+// tiles give each tile to the four warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
+// stages of its own with 16-byte asynchronous copies.
 #include "kv8.cuh"
 
 namespace liger {
@@ -28,7 +29,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 16;            // keys of a step
-constexpr int kMinSteps = 16;        // steps that are worth a CTA
+constexpr int kTileCost = 4;         // what it costs to begin a tile, in steps
+constexpr int kMinPlaces = 8;        // places that are worth a warp
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -40,19 +42,25 @@ struct AttnParams {
   long long q_batch_stride, q_token_stride, q_head_stride;
   int heads, group, max_kv_len, ldo, causal;
   float scale_log2;
-  int whole_tiles;   // 1: CTA = tile (grid: tiles of an entry, entries); 0: equal shares of the line
   int tiles;         // most tiles of an entry
-  float* parts;      // [2 * CTAs] partial results
+  // shares
+  int workers;       // warps of the launch
+  int by_tile;       // 1: records are numbered by entry and tile, 0: by the worker that began the tile
+  int2* records;     // a tile that is split: the workers that have its first and its last part (else x = -1)
+  int4* tile_of;     // by worker only: the entry, tile of that record
+  float* parts;      // [2 * workers] partial results
   DeviceStatus* status;
 };
 
 template <int D, int NT>
 struct Cfg {
   static constexpr int kRows = 8 * NT;
+  static constexpr int kCtas = NT == 1 ? 3 : 2;                      // resident per SM
   static constexpr int kStage = 2 * kStep * D;                       // K and V of a step
-  static constexpr int kStages = D == 128 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 12 : 8);
-  static constexpr int kMerge = kWarps * kRows * (D + 4) * 4;        // accumulators of the warps
-  static constexpr int kSmem = kWarps * kStages * kStage + kMerge;
+  static constexpr int kStages = (NT == 1 ? 4 : 6) * (128 / D);
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kMerge = kWarps * kRows * (D + 4) * 4;        // accumulators of a CTA's warps, in the place of the rings
+  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
   static constexpr int kPart = kRows * (D + 2);                      // floats of a partial result: maxima, sums, accumulators
 };
 
@@ -95,66 +103,77 @@ template <int ROWS>
 __device__ __forceinline__ int row_tiles(const AttnParams& p, const Entry& e) { return (e.n * p.group + ROWS - 1) / ROWS; }
 // an entry without keys still has rows to fill with zeros
 __device__ __forceinline__ int steps_of(const Entry& e) { return max(1, (e.len + kStep - 1) / kStep); }
+__device__ __forceinline__ int places_of(const Entry& e) { return steps_of(e) + kTileCost; }
 template <int ROWS>
 __device__ __forceinline__ long long line_of(const AttnParams& p, const Entry& e) {
-  return (long long)p.c.kv_heads * row_tiles<ROWS>(p, e) * steps_of(e);
+  return (long long)p.c.kv_heads * row_tiles<ROWS>(p, e) * places_of(e);
 }
 
-__device__ __forceinline__ int ctas_used(long long total, int ctas) {
-  const long long want = (total + kMinSteps - 1) / kMinSteps;
-  return (int)(want < ctas ? want : ctas);
+__device__ __forceinline__ int workers_used(long long total, int workers) {
+  const long long want = (total + kMinPlaces - 1) / kMinPlaces;
+  return (int)(want < workers ? want : workers);
 }
-__device__ __forceinline__ long long share_begin(long long total, int used, int cta) { return total * cta / used; }
-__device__ __forceinline__ int share_of(long long total, int used, long long at) {  // the CTA whose share has step `at`
-  int c = (int)(at * used / total);
-  while (share_begin(total, used, c + 1) <= at) ++c;
-  while (share_begin(total, used, c) > at) --c;
-  return c;
+__device__ __forceinline__ long long share_begin(long long total, int used, int w) { return total * w / used; }
+__device__ __forceinline__ int share_of(long long total, int used, long long at) {  // the worker whose share has place `at`
+  int w = (int)(at * used / total);
+  while (share_begin(total, used, w + 1) <= at) ++w;
+  while (share_begin(total, used, w) > at) --w;
+  return w;
 }
 
-// Sum over the entries, and the entry that has place `at` of the line (at = f(total)); all threads of the CTA get the answer.
-template <int ROWS, int THREADS, typename F>
-__device__ __forceinline__ void find_place(const AttnParams& p, F place, long long& total, long long& at, int& b_out, long long& b_first) {
-  __shared__ long long s_warp[THREADS / 32], s_first;
-  __shared__ int s_b;
+// The line's length, and for each warp of the CTA the entry in which its share begins and that entry's first place (entry -1:
+// the warp has no share).
+template <int ROWS>
+__device__ __forceinline__ void find_shares(const AttnParams& p, long long& total, int& used, int& b_out, long long& b_first) {
+  __shared__ long long s_warp[kWarps], s_first[kWarps];
+  __shared__ int s_b[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long mine = 0;
-  for (int b = threadIdx.x; b < p.e.batch; b += THREADS) mine += line_of<ROWS>(p, load_entry(p, b, false));
+  for (int b = threadIdx.x; b < p.e.batch; b += kThreads) mine += line_of<ROWS>(p, load_entry(p, b, blockIdx.x == 0));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) s_warp[warp] = mine;
-  if (threadIdx.x == 0) s_b = -1;
+  if (threadIdx.x < kWarps) s_b[threadIdx.x] = -1;
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) total += s_warp[w];
-  at = place(total);
+  for (int w = 0; w < kWarps; ++w) total += s_warp[w];
+  used = workers_used(total, p.workers);
   __syncthreads();
-  if (at < 0 || at >= total) { b_out = -1; return; }  // the same in all threads
-  long long before = 0;
-  for (int base = 0; base < p.e.batch; base += THREADS) {
-    const int b = base + threadIdx.x;
-    const long long v = b < p.e.batch ? line_of<ROWS>(p, load_entry(p, b, false)) : 0;
-    long long incl = v;
+  const int w0 = blockIdx.x * kWarps;
+  if (w0 < used) {
+    const long long last = share_begin(total, used, min(w0 + kWarps, used) - 1);  // where the last of the CTA's shares begins
+    long long before = 0;
+    for (int base = 0; base < p.e.batch && before <= last; base += kThreads) {
+      const int b = base + threadIdx.x;
+      const long long v = b < p.e.batch ? line_of<ROWS>(p, load_entry(p, b, false)) : 0;
+      long long incl = v;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) s_warp[warp] = incl;
+      __syncthreads();
+      long long all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) incl += s_warp[w];
+        all += s_warp[w];
+      }
+      const long long lo = before + incl - v, hi = before + incl;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w0 + w >= used) break;
+        const long long at = share_begin(total, used, w0 + w);
+        if (at >= lo && at < hi) { s_b[w] = b; s_first[w] = lo; }
+      }
+      before += all;
+      __syncthreads();
     }
-    if (lane == 31) s_warp[warp] = incl;
-    __syncthreads();
-    long long all = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) incl += s_warp[w];
-      all += s_warp[w];
-    }
-    if (at >= before + incl - v && at < before + incl) { s_b = b; s_first = before + incl - v; }
-    before += all;
-    __syncthreads();
-    if (s_b >= 0) break;
   }
-  b_out = s_b;
-  b_first = s_first;
+  b_out = s_b[warp];
+  b_first = s_first[warp];
 }
 
 // 16-byte chunk `c` of key `r` of a step.  The xor spreads both ways of reading over all banks: a lane quad reads a key
@@ -165,54 +184,61 @@ __device__ __forceinline__ int stage_at(int r, int c) {
   return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (r & 6)) << 4);  // two keys a line
 }
 
-template <int D, int TYPE, int NT>
-__global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnParams p) {
+template <int D, int TYPE, int NT, int WHOLE>
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_kernel(const AttnParams p) {
   using C = Cfg<D, NT>;
-  constexpr int kKk = D / 16;             // k-steps of a score product = dim tiles of an output product
+  constexpr int kKk = D / 16;                     // k-steps of a score product = dim tiles of an output product
+  constexpr int kStride = WHOLE ? kWarps : 1;     // the warps of a whole tile take every fourth step
   extern __shared__ __align__(128) uint8_t smem_kv8[];
-  __shared__ float s_m[kWarps][C::kRows], s_l[kWarps][C::kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_kv8 + warp * C::kStages * C::kStage;
   const uint32_t ring_u = smem_u32(ring);
-  float* merge = reinterpret_cast<float*>(smem_kv8 + kWarps * C::kStages * C::kStage);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // this CTA's share: places [at, end) of the line, beginning in entry b whose places start at b_first
+  // the places [at, end) of the line, beginning in entry b whose places start at b_first
   long long total = 0, at = 0, end = 0, b_first = 0;
   int b, used = 0;
-  const int cta = blockIdx.x;
+  const int worker = blockIdx.x * kWarps + warp;
   Entry e;
-  if (p.whole_tiles) {
+  if (WHOLE) {
     b = blockIdx.y;
     e = load_entry(p, b, blockIdx.x == 0 && threadIdx.x == 0);
-    const int tile = blockIdx.x;
-    if (tile >= p.c.kv_heads * row_tiles<C::kRows>(p, e)) return;
-    at = (long long)tile * steps_of(e);
-    end = at + steps_of(e);
+    if ((int)blockIdx.x >= p.c.kv_heads * row_tiles<C::kRows>(p, e)) return;
+    at = (long long)blockIdx.x * places_of(e);
+    end = at + places_of(e);
   } else {
-    if (cta == 0)
-      for (int i = threadIdx.x; i < p.e.batch; i += kThreads) load_entry(p, i, true);
-    find_place<C::kRows, kThreads>(
-        p, [&](long long all) {
-          used = ctas_used(all, gridDim.x);
-          return cta < used ? share_begin(all, used, cta) : -1;
-        },
-        total, at, b, b_first);
+    find_shares<C::kRows>(p, total, used, b, b_first);
+    if (!p.by_tile && lane == 0) p.records[worker].x = -1;
     if (b < 0) return;
-    end = share_begin(total, used, cta + 1);
+    at = share_begin(total, used, worker);
+    end = share_begin(total, used, worker + 1);
     e = load_entry(p, b, false);
   }
   const long long share0 = at;
 
   while (at < end) {
-    const int steps = steps_of(e);
-    const long long inside = at - b_first;
-    const int tile = (int)(inside / steps), s_begin = (int)(inside % steps);
+    const int steps = steps_of(e), places = places_of(e);
+    const int tile = (int)((at - b_first) / places), place = (int)((at - b_first) % places);
+    const int left = (int)((long long)(places - place) < end - at ? places - place : end - at);  // places of the share in this tile
     const int tiles = row_tiles<C::kRows>(p, e);
     const int head = tile / tiles, row_base = (tile % tiles) * C::kRows;
-    const int s_end = (int)((long long)steps < s_begin + (end - at) ? steps : s_begin + (end - at));
+    // a share that ends before a tile's first step leaves the tile to the next
+    const int s_begin = max(0, place - kTileCost), s_end = max(0, place + left - kTileCost);
     const int rows = e.n * p.group;
+    const bool complete = s_begin == 0 && s_end == steps;
+    if (!WHOLE && lane == 0) {
+      // who begins a tile knows who ends it
+      int2* rec = nullptr;
+      if (s_begin == 0 && s_end > 0) rec = p.records + (p.by_tile ? (size_t)b * p.tiles + tile : (size_t)worker);
+      if (rec && (p.by_tile || !complete)) {
+        const long long t1 = b_first + (long long)(tile + 1) * places;
+        *rec = complete ? make_int2(-1, 0) : make_int2(worker, share_of(total, used, t1 - 1));
+        if (!p.by_tile) p.tile_of[worker] = make_int4(b, tile, 0, 0);
+      }
+    }
 
+   if (s_end > 0) {
     // this lane's rows: as B operand row g of each n-tile, as accumulator column 2t, 2t + 1
     uint32_t qf[NT][kKk][2];
     int limit[NT][2], limit_min = e.len;
@@ -256,8 +282,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnPa
       for (int i = 0; i < kKk; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f; }
     }
 
-    // this warp's steps: s_begin + warp + i * kWarps, i < count (an entry without keys has none)
-    const int count = e.len > 0 && s_begin + warp < s_end ? (s_end - s_begin - warp + kWarps - 1) / kWarps : 0;
+    // this warp's steps: s_first + i * kStride, i < count (an entry without keys has none)
+    const int s_first = s_begin + (WHOLE ? warp : 0);
+    const int count = e.len > 0 && s_first < s_end ? (s_end - s_first + kStride - 1) / kStride : 0;
     const int* row_table = p.c.table + (size_t)e.slot * p.c.max_pages;
     const int page_mask = (1 << p.c.page_shift) - 1;
     // page and scales of 32 steps, one per lane: `now` for steps being copied, the lookups of the next 32 under way
@@ -266,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnPa
       page = -1;
       ks = vs = 0.0f;
       if (i < count) {
-        const int key = (s_begin + warp + i * kWarps) * kStep;
+        const int key = (s_first + i * kStride) * kStep;
         page = __ldg(row_table + (key >> p.c.page_shift));
         if (page < 0 || page >= p.c.num_pages) {
           report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 2, b, (unsigned)page);
@@ -289,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnPa
       if (i < count) {
         const int page = __shfl_sync(0xffffffffu, (i >> 5) & 1 ? page_odd : page_even, i & 31);
         if (page >= 0) {
-          const int key = (s_begin + warp + i * kWarps) * kStep;
+          const int key = (s_first + i * kStride) * kStep;
           const size_t src = ((((size_t)page * p.c.kv_heads + head) << p.c.page_shift) + (key & page_mask)) * D;
           const uint32_t dst = ring_u + (i % C::kStages) * C::kStage;
           constexpr int kChunks = D / 16;
@@ -320,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnPa
       const int page = __shfl_sync(0xffffffffu, odd ? page_odd : page_even, i & 31);
       const float ks = __shfl_sync(0xffffffffu, odd ? ks_odd : ks_even, i & 31);
       const float vs = __shfl_sync(0xffffffffu, odd ? vs_odd : vs_even, i & 31);
-      const int key0 = (s_begin + warp + i * kWarps) * kStep;
+      const int key0 = (s_first + i * kStride) * kStep;
       const uint8_t* sk = ring + (i % C::kStages) * C::kStage;
       uint8_t* sv = ring + (i % C::kStages) * C::kStage + kStep * D;
       if (page >= 0) {
@@ -445,58 +472,83 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnPa
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-    // join the warps
-    float m_w[NT][2];
+    // this warp's sums over the keys' lanes
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float l = l_run[nt][c];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        m_w[nt][c] = m_ref[nt][c];
-        const int r = nt * 8 + 2 * t + c;
-        if (g == 0) { s_m[warp][r] = m_w[nt][c]; s_l[warp][r] = l; }
-        float* dst = merge + (warp * C::kRows + r) * (D + 4) + g * (D / 8);
-#pragma unroll
-        for (int d = 0; d < kKk; d += 2)
-          *reinterpret_cast<float4*>(dst + 2 * d) = make_float4(o[nt][d][c] * v_ref, o[nt][d][c + 2] * v_ref, o[nt][d + 1][c] * v_ref, o[nt][d + 1][c + 2] * v_ref);
+        l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 4);
+        l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 8);
+        l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 16);
       }
-    }
-    __syncthreads();
-    const bool complete = s_begin == 0 && s_end == steps;
-    float* part = p.parts + (size_t)(2 * cta + (at == share0 && s_begin > 0 ? 0 : 1)) * C::kPart;
-    for (int i = threadIdx.x; i < C::kRows * D / 4; i += kThreads) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      if (row_base + r >= rows) continue;
-      float m = s_m[0][r];
+    if (WHOLE) {
+      __shared__ float s_m[kWarps][C::kRows], s_l[kWarps][C::kRows];
+      float* merge = reinterpret_cast<float*>(smem_kv8);
+      __syncthreads();  // the rings are done with
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][r]);
-      float l = 0.0f;
-      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float lw = s_l[w][r];
-        const float f = lw == 0.0f ? 0.0f : lw == lw ? exp2_approx(s_m[w][r] - m) : 1.0f;  // saw nothing / a NaN stays
-        const float4 x = *reinterpret_cast<const float4*>(merge + (w * C::kRows + r) * (D + 4) + d);
-        l += f * lw;
-        a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
-      }
-      if (complete) {
+        for (int c = 0; c < 2; ++c) {
+          const int r = nt * 8 + 2 * t + c;
+          if (g == 0) { s_m[warp][r] = m_ref[nt][c]; s_l[warp][r] = l_run[nt][c]; }
+          float* dst = merge + (warp * C::kRows + r) * (D + 4) + g * (D / 8);
+#pragma unroll
+          for (int d = 0; d < kKk; d += 2)
+            *reinterpret_cast<float4*>(dst + 2 * d) = make_float4(o[nt][d][c] * v_ref, o[nt][d][c + 2] * v_ref, o[nt][d + 1][c] * v_ref, o[nt][d + 1][c + 2] * v_ref);
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < C::kRows * D / 4; i += kThreads) {
+        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (row_base + r >= rows) break;
+        float m = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][r]);
+        float l = 0.0f;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float lw = s_l[w][r];
+          const float f = lw == 0.0f ? 0.0f : lw == lw ? exp2_approx(s_m[w][r] - m) : 1.0f;  // saw nothing / a NaN stays
+          const float4 x = *reinterpret_cast<const float4*>(merge + (w * C::kRows + r) * (D + 4) + d);
+          l += f * lw;
+          a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+        }
         const int token = (row_base + r) / p.group;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         __half* dst = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + (row_base + r) % p.group) * D + d;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2(a.x * inv, a.y * inv), pack_half2(a.z * inv, a.w * inv));
-      } else {
-        if (d == 0) { part[r] = m; part[C::kRows + r] = l; }
-        *reinterpret_cast<float4*>(part + 2 * C::kRows + r * D + d) = a;
       }
+      return;
     }
-    __syncthreads();
+    float* part = p.parts + (size_t)(2 * worker + (at == share0 && s_begin > 0 ? 0 : 1)) * C::kPart;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = nt * 8 + 2 * t + c;
+        if (row_base + r >= rows) continue;
+        if (complete) {
+          const int token = (row_base + r) / p.group;
+          const float inv = l_run[nt][c] == 0.0f ? 0.0f : v_ref / l_run[nt][c];
+          __half* dst = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + (row_base + r) % p.group) * D + g * (D / 8);
+#pragma unroll
+          for (int d = 0; d < kKk; d += 4)
+            *reinterpret_cast<uint4*>(dst + 2 * d) = make_uint4(pack_half2(o[nt][d][c] * inv, o[nt][d][c + 2] * inv),
+                                                                pack_half2(o[nt][d + 1][c] * inv, o[nt][d + 1][c + 2] * inv),
+                                                                pack_half2(o[nt][d + 2][c] * inv, o[nt][d + 2][c + 2] * inv),
+                                                                pack_half2(o[nt][d + 3][c] * inv, o[nt][d + 3][c + 2] * inv));
+        } else {
+          if (g == 0) { part[r] = m_ref[nt][c]; part[C::kRows + r] = l_run[nt][c]; }
+          float* dst = part + 2 * C::kRows + r * D + g * (D / 8);
+#pragma unroll
+          for (int d = 0; d < kKk; d += 2)
+            *reinterpret_cast<float4*>(dst + 2 * d) = make_float4(o[nt][d][c] * v_ref, o[nt][d][c + 2] * v_ref, o[nt][d + 1][c] * v_ref, o[nt][d + 1][c + 2] * v_ref);
+        }
+      }
+   }
 
-    at += s_end - s_begin;
-    if (at < end && at == b_first + (long long)p.c.kv_heads * tiles * steps) {
+    at += left;
+    if (at < end && at == b_first + (long long)p.c.kv_heads * tiles * places) {
       b_first = at;
       do {
         ++b;
@@ -508,38 +560,38 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attention_kernel(const AttnPa
 
 constexpr int kJoinThreads = 256;
 
-// Joins the parts of the tiles that more than one CTA worked on.  CTA (c, r) has row r of the tile that lies across the border
-// between shares c and c + 1, where that is the tile's first border.
+// Joins the parts of the tiles that are split over several shares: CTA (record, row).
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const AttnParams p, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const AttnParams p) {
   using C = Cfg<D, NT>;
   constexpr int kW = kJoinThreads / 32;
   __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
-  const int border = blockIdx.x + 1, r = blockIdx.y;
-  long long total, at, b_first;
-  int b, used = 0;
-  find_place<C::kRows, kJoinThreads>(
-      p, [&](long long all) {
-        used = ctas_used(all, ctas);
-        return border < used ? share_begin(all, used, border) : -1;
-      },
-      total, at, b, b_first);
-  if (b < 0) return;
-  const Entry e = load_entry(p, b, false);
-  const int steps = steps_of(e), tiles = row_tiles<C::kRows>(p, e);
-  const int tile = (int)((at - b_first) / steps);
-  const long long t0 = b_first + (long long)tile * steps, t1 = t0 + steps;
-  if (t0 == at || share_begin(total, used, border - 1) > t0) return;  // nothing across this border, or not the first border
-  const int c0 = border - 1, c1 = share_of(total, used, t1 - 1);
+  const int r = blockIdx.y;
+  int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  Entry e;
+  if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel
+  // every CTA waits, also one that has nothing to do: what follows on the stream counts on the first kernel's end
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.by_tile && tile >= p.c.kv_heads * row_tiles<C::kRows>(p, e)) return;
+  const int2 rec = p.records[blockIdx.x];
+  if (rec.x < 0) return;
+  if (!p.by_tile) {
+    const int4 at = p.tile_of[blockIdx.x];
+    b = at.x;
+    tile = at.y;
+    e = load_entry(p, b, false);
+  }
+  const int tiles = row_tiles<C::kRows>(p, e);
   const int head = tile / tiles, row = (tile % tiles) * C::kRows + r;
   if (row >= e.n * p.group) return;
-  // shares c0 .. c1; the first one began the tile (unless its share began with it, that is its second slot)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float m = -INFINITY, l = 0.0f, a[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) a[i] = 0.0f;
-  for (int c = c0 + warp; c <= c1; c += kW) {
-    const float* part = p.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * C::kPart;
+#pragma unroll 4
+  for (int c = rec.x + warp; c <= rec.y; c += kW) {
+    // the first part is its worker's last tile, the others are their workers' first
+    const float* part = p.parts + (size_t)(2 * c + (c == rec.x ? 1 : 0)) * C::kPart;
     const float pm = part[r], pl = part[C::kRows + r];
     float x[D / 32];
     if (D == 128) {
@@ -549,9 +601,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
       const float2 v = *reinterpret_cast<const float2*>(part + 2 * C::kRows + r * D + lane * 2);
       x[0] = v.x; x[1] = v.y;
     }
-    if (pl == 0.0f) continue;  // saw nothing
-    const float m_new = fmaxf(m, pm);
-    const float fa = m == -INFINITY ? 0.0f : exp2_approx(m - m_new), fb = exp2_approx(pm - m_new);
+    const float m_new = pl == 0.0f ? m : fmaxf(m, pm);  // a part that saw nothing changes nothing
+    const float fa = l == 0.0f ? 0.0f : exp2_approx(m - m_new), fb = pl == 0.0f ? 0.0f : exp2_approx(pm - m_new);
     m = m_new;
     l = l * fa + pl * fb;
 #pragma unroll
@@ -578,39 +629,54 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
 }
 
 struct Plan {
-  int nt, rows, tiles, whole_tiles, ctas;
-  size_t part_floats;
+  int nt, rows, live, tiles, whole, workers, by_tile, records;
+  size_t bytes;  // of scratch
 };
 
-// How a call is launched; a function of its sizes alone.
+// How a call is launched; a function of its sizes and the SM count alone.
 Plan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm_count) {
   Plan p;
   const long long rows = (long long)a->q_len * (a->heads / c->kv_heads);
-  p.nt = rows > 8 ? 2 : 1;
+  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
   p.rows = 8 * p.nt;
+  p.live = (int)(rows < p.rows ? rows : p.rows);
   const long long tiles = (long long)c->kv_heads * ((rows + p.rows - 1) / p.rows);
   p.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
-  p.whole_tiles = a->max_kv_len <= 512;
-  p.ctas = 2 * sm_count;
-  p.part_floats = p.whole_tiles ? 0 : (size_t)2 * p.ctas * p.rows * (c->head_dim + 2);
+  const int ctas = (p.nt == 1 ? 3 : 2) * sm_count;
+  p.whole = a->max_kv_len <= 1024 && tiles * a->batch <= ctas;
+  p.workers = ctas * kWarps;
+  p.by_tile = tiles * a->batch <= p.workers;
+  p.records = p.by_tile ? p.tiles * a->batch : p.workers;
+  p.bytes = p.whole ? 0 : (size_t)p.workers * (sizeof(int2) + sizeof(int4)) + (size_t)2 * p.workers * p.rows * (c->head_dim + 2) * sizeof(float);
   return p;
 }
 
-template <int D, int TYPE, int NT>
+template <int D, int TYPE, int NT, int WHOLE>
 int launch(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
   using C = Cfg<D, NT>;
-  LIGER_CUDA_TRY(cudaFuncSetAttribute(kv8_attention_kernel<D, TYPE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  const dim3 grid = pl.whole_tiles ? dim3(pl.tiles, ap.e.batch) : dim3(pl.ctas);
-  kv8_attention_kernel<D, TYPE, NT><<<grid, kThreads, C::kSmem, s>>>(ap);
+  LIGER_CUDA_TRY(cudaFuncSetAttribute(kv8_attention_kernel<D, TYPE, NT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  const dim3 grid = WHOLE ? dim3(pl.tiles, ap.e.batch) : dim3(pl.workers / kWarps);
+  kv8_attention_kernel<D, TYPE, NT, WHOLE><<<grid, kThreads, C::kSmem, s>>>(ap);
   int rc = check_launch("kv8_attention_kernel");
-  if (rc != LIGER_OK || pl.whole_tiles) return rc;
-  kv8_attention_join_kernel<D, NT><<<dim3(pl.ctas - 1, pl.rows), kJoinThreads, 0, s>>>(ap, pl.ctas);
-  return check_launch("kv8_attention_join_kernel");
+  if (rc != LIGER_OK || WHOLE) return rc;
+  // launched while the first kernel runs; waits for it on the device
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(pl.records, pl.live);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  LIGER_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_join_kernel<D, NT>, ap));
+  return LIGER_OK;
 }
 
 template <int D, int TYPE>
 int launch_rows(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
-  return pl.nt == 1 ? launch<D, TYPE, 1>(ap, pl, s) : launch<D, TYPE, 2>(ap, pl, s);
+  if (pl.whole) return pl.nt == 1 ? launch<D, TYPE, 1, 1>(ap, pl, s) : pl.nt == 2 ? launch<D, TYPE, 2, 1>(ap, pl, s) : launch<D, TYPE, 3, 1>(ap, pl, s);
+  return pl.nt == 1 ? launch<D, TYPE, 1, 0>(ap, pl, s) : pl.nt == 2 ? launch<D, TYPE, 2, 0>(ap, pl, s) : launch<D, TYPE, 3, 0>(ap, pl, s);
 }
 
 int check_args(const liger_kv8_cache* c, const liger_kv8_attention_args* a) {
@@ -647,7 +713,7 @@ extern "C" size_t liger_kv8_attention_scratch_bytes(const liger_kv8_cache* cache
     cudaGetLastError();
     sms = kAssumedSms;
   }
-  return plan_of(cache, args, sms).part_floats * sizeof(float);
+  return plan_of(cache, args, sms).bytes;
 }
 
 extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8_attention_args* a, void* stream) {
@@ -658,13 +724,12 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
     return set_error(LIGER_ERR_INVALID, "kv8_attention: q, out and scratch must be 16-byte aligned");
   if (((uintptr_t)a->kv_lens | (uintptr_t)a->slots) & 3u)
     return set_error(LIGER_ERR_INVALID, "kv8_attention: kv_lens and slots must be 4-byte aligned");
-  if (!a->scratch && plan_of(cache, a, kAssumedSms).part_floats) return set_error(LIGER_ERR_INVALID, "kv8_attention: scratch is NULL");
+  if (!a->scratch && plan_of(cache, a, kAssumedSms).bytes) return set_error(LIGER_ERR_INVALID, "kv8_attention: scratch is NULL");
   const DeviceInfo* dev = current_device();
   if (!dev) return LIGER_ERR_CUDA;
   const Plan pl = plan_of(cache, a, dev->sm_count);
-  const size_t need = pl.part_floats * sizeof(float);
-  if (a->scratch_bytes < need)
-    return set_error(LIGER_ERR_TOO_LARGE, "kv8_attention: scratch has %zu bytes, %zu are needed", a->scratch_bytes, need);
+  if (a->scratch_bytes < pl.bytes)
+    return set_error(LIGER_ERR_TOO_LARGE, "kv8_attention: scratch has %zu bytes, %zu are needed", a->scratch_bytes, pl.bytes);
   if (pl.tiles == 0x7fffffff) return set_error(LIGER_ERR_UNSUPPORTED, "kv8_attention: q_len %d x heads %d is too large", a->q_len, a->heads);
   AttnParams p{};
   p.c = kv8_layer(cache, a->layer);
@@ -681,9 +746,12 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   p.ldo = a->ldo;
   p.causal = a->causal;
   p.scale_log2 = a->scale * kLog2e;
-  p.whole_tiles = pl.whole_tiles;
   p.tiles = pl.tiles;
+  p.workers = pl.workers;
+  p.by_tile = pl.by_tile;
   p.parts = (float*)a->scratch;
+  p.tile_of = (int4*)(p.parts + (size_t)2 * pl.workers * pl.rows * (cache->head_dim + 2));
+  p.records = (int2*)(p.tile_of + pl.workers);
   p.status = dev->status_dev;
   cudaStream_t s = (cudaStream_t)stream;
   if (cache->head_dim == 128)
