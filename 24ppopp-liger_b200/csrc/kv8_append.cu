@@ -1,9 +1,10 @@
 // Writing new keys and values into the paged 8-bit cache (liger_kv8_append), and the argument checks of its operators.
 //
 // A unit of work is one block of `scale_block` tokens of one head, keys or values.  Its threads hold all of the block's new
-// values in registers (64 per thread), so that the values are read once: the largest magnitude is found with integer maxima
-// on the fp16 bit patterns (for non-negative numbers the order of the patterns is the order of the values, and a NaN is above
-// infinity, so that it is not lost), then the codes are rounded and written.  The codes that a block already holds are only read
+// values in registers (64 per thread), so that the values are read once: the largest magnitude is found with fp16
+// maxima that keep a NaN (and between lanes with integer maxima of the bit patterns, in which a NaN is above infinity), then the
+// codes are rounded and written.  A new value times the reciprocal is at most the largest code * (1 + 2^-22), so it rounds to
+// a code without a bound.  The codes that a block already holds are only read
 // when its scale grows.
 #include "kv8.cuh"
 
@@ -85,6 +86,15 @@ struct AppendParams {
   DeviceStatus* status;
 };
 
+// Codes of a block whose scale grows.  The ratio is at most 1 (to rounding); a code -128 that somebody else wrote becomes -127.
+template <int TYPE>
+__device__ __forceinline__ uint32_t encode_held(const float (&f)[4], float ratio) {
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = TYPE == LIGER_KV8_INT8 ? fmaxf(f[i] * ratio, -127.0f) : f[i] * ratio;
+  return kv8_encode4<TYPE>(y[0], y[1], y[2], y[3]);
+}
+
 // Grid: (units of an entry / units of a CTA, entries).  Units are ordered heads first, so that neighbouring warps read
 // neighbouring runs of the source's rows.
 template <int D, int TYPE, int U>
@@ -120,7 +130,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   const int blk = rest % p.blocks, is_v = rest / p.blocks;
   const int block0 = pos0 >> p.c.block_shift;            // the first block that is touched
   const int start = (block0 + blk) << p.c.block_shift;   // this unit's first position
-  bool active = is_v < 2 && start < pos0 + n;
+  const bool wanted = is_v < 2 && start < pos0 + n;
+  bool active = wanted;
   int page = -1;
   if (active) {
     page = __ldg(p.c.table + (size_t)slot * p.c.max_pages + (start >> p.c.page_shift));
@@ -140,17 +151,29 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   const bool goes_on = active && held > 0;
   const float s_old = goes_on ? *scale : 0.0f;
 
+  // the thread's pieces: piece `piece` of rows r0, r0 + rows_u, ...
+  const int piece = t % kPieces, r0 = t / kPieces, rows_u = p.unit / kPieces;
+  const int r_end = min(end, 1 << p.c.block_shift);
   uint4 x[U];
-  uint32_t mx = 0;
+  __half2 hm = __half2half2(__ushort_as_half(0));
+  {
+    const __half* at = src + (long long)(start + r0 - pos0) * p.token_stride + piece * 8;
+    const long long step = (long long)rows_u * p.token_stride;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * rows_u;
+      x[u] = make_uint4(0, 0, 0, 0);
+      if (wanted && r >= held && r < r_end) x[u] = __ldcs(reinterpret_cast<const uint4*>(at + u * step));
+    }
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = u * p.unit + t, r = i / kPieces, piece = i % kPieces;
-    x[u] = make_uint4(0, 0, 0, 0);
-    if (active && r >= held && r < end && r < (1 << p.c.block_shift))
-      x[u] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)(start + r - pos0) * p.token_stride + piece * 8));
-    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu), __vmaxu2(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu)));
+    const __half2* h = reinterpret_cast<const __half2*>(&x[u]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) hm = __hmax2_nan(hm, __habs2(h[j]));
   }
-  mx = __reduce_max_sync(0xffffffffu, max(mx & 0xffffu, mx >> 16));
+  const uint32_t hb = *reinterpret_cast<const uint32_t*>(&hm);
+  uint32_t mx = __reduce_max_sync(0xffffffffu, max(hb & 0xffffu, hb >> 16));
   if (p.unit > 32) {  // the same for the whole grid
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) s_max[warp] = mx;
@@ -168,7 +191,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     const float ratio = s_old * back;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = u * p.unit + t, r = i / kPieces, piece = i % kPieces;
+      const int r = r0 + u * rows_u;
       if (r < held && r < (1 << p.c.block_shift)) {
         uint2* at = reinterpret_cast<uint2*>(codes + (size_t)r * D + piece * 8);
         uint2 c = make_uint2(0, 0);
@@ -176,9 +199,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
           c = *at;
           float f[4];
           kv8_decode4<TYPE>(c.x, f);
-          c.x = kv8_encode4<TYPE>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+          c.x = encode_held<TYPE>(f, ratio);
           kv8_decode4<TYPE>(c.y, f);
-          c.y = kv8_encode4<TYPE>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+          c.y = encode_held<TYPE>(f, ratio);
         }
         *at = c;
       }
@@ -186,8 +209,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = u * p.unit + t, r = i / kPieces, piece = i % kPieces;
-    if (r >= held && r < end && r < (1 << p.c.block_shift)) {
+    const int r = r0 + u * rows_u;
+    if (r >= held && r < r_end) {
       uint2 c = make_uint2(0, 0);
       if (finite) {
         float f[8];

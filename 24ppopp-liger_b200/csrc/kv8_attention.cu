@@ -560,13 +560,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_ker
 
 constexpr int kJoinThreads = 256;
 
-// Joins the parts of the tiles that are split over several shares: CTA (record, row).
+// Joins the parts of the tiles that are split over several shares.  A CTA has the rows [blockIdx.y * rows_cta, ..) of a tile:
+// one row for its eight warps where there are few tiles, which are then split into many parts, else eight rows, one a warp.
+// The parts' maxima and sums are looked at first, 32 at a time, so that the accumulators are read without waiting for one another.
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const AttnParams p, int rows_cta) {
   using C = Cfg<D, NT>;
-  constexpr int kW = kJoinThreads / 32;
+  constexpr int kW = kJoinThreads / 32, kA = D / 32;
   __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
-  const int r = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
   Entry e;
   if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel
@@ -581,50 +583,76 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
     tile = at.y;
     e = load_entry(p, b, false);
   }
+  const bool shared = rows_cta == 1;
+  const int r = shared ? blockIdx.y : blockIdx.y * rows_cta + warp;
   const int tiles = row_tiles<C::kRows>(p, e);
   const int head = tile / tiles, row = (tile % tiles) * C::kRows + r;
-  if (row >= e.n * p.group) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float m = -INFINITY, l = 0.0f, a[D / 32];
+  if (r >= C::kRows || row >= e.n * p.group) return;  // the whole CTA where it shares a row
+  const int first = rec.x + (shared ? warp : 0), stride = shared ? kW : 1;
+  const int parts = rec.y >= first ? (rec.y - first) / stride + 1 : 0;
+  // the first part is its worker's last tile, the others are their workers' first
+  auto part_of = [&](int i) {
+    const int w = first + i * stride;
+    return p.parts + (size_t)(2 * w + (w == rec.x ? 1 : 0)) * C::kPart;
+  };
+  float m = -INFINITY, l = 0.0f, a[kA];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) a[i] = 0.0f;
-#pragma unroll 4
-  for (int c = rec.x + warp; c <= rec.y; c += kW) {
-    // the first part is its worker's last tile, the others are their workers' first
-    const float* part = p.parts + (size_t)(2 * c + (c == rec.x ? 1 : 0)) * C::kPart;
-    const float pm = part[r], pl = part[C::kRows + r];
-    float x[D / 32];
-    if (D == 128) {
-      const float4 v = *reinterpret_cast<const float4*>(part + 2 * C::kRows + r * D + lane * 4);
-      x[0] = v.x; x[1] = v.y; x[2 % (D / 32)] = v.z; x[3 % (D / 32)] = v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(part + 2 * C::kRows + r * D + lane * 2);
-      x[0] = v.x; x[1] = v.y;
+  for (int i = 0; i < kA; ++i) a[i] = 0.0f;
+  for (int base = 0; base < parts; base += 32) {
+    float pm = -INFINITY, pl = 0.0f;
+    if (base + lane < parts) {
+      const float* q = part_of(base + lane);
+      pm = __ldcg(q + r);
+      pl = __ldcg(q + C::kRows + r);
     }
-    const float m_new = pl == 0.0f ? m : fmaxf(m, pm);  // a part that saw nothing changes nothing
-    const float fa = l == 0.0f ? 0.0f : exp2_approx(m - m_new), fb = pl == 0.0f ? 0.0f : exp2_approx(pm - m_new);
+    const float m_new = fmaxf(m, warp_max(pl == 0.0f ? -INFINITY : pm));
+    // a part that saw nothing has no weight; a NaN stays
+    const float f = pl == 0.0f ? 0.0f : pl == pl ? exp2_approx(pm - m_new) : 1.0f;
+    const float fa = l == 0.0f ? 0.0f : l == l ? exp2_approx(m - m_new) : 1.0f;
     m = m_new;
-    l = l * fa + pl * fb;
+    l = l * fa + warp_sum(f * pl);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) a[i] = a[i] * fa + x[i] * fb;
+    for (int i = 0; i < kA; ++i) a[i] *= fa;
+    const int n = min(32, parts - base);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+      const float* q = part_of(base + j) + 2 * C::kRows + r * D + lane * kA;
+      if (D == 128) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(q));
+        a[0] += v.x * fj; a[1] += v.y * fj; a[2 % kA] += v.z * fj; a[3 % kA] += v.w * fj;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
+        a[0] += v.x * fj; a[1] += v.y * fj;
+      }
+    }
+  }
+  const int token = row / p.group;
+  __half* out = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
+  if (!shared) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (D == 128)
+      *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack_half2(a[0] * inv, a[1] * inv), pack_half2(a[2 % kA] * inv, a[3 % kA] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out + lane * 2) = pack_half2(a[0] * inv, a[1] * inv);
+    return;
   }
   if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) s_a[warp][lane * (D / 32) + i] = a[i];
+  for (int i = 0; i < kA; ++i) s_a[warp][lane * kA + i] = a[i];
   __syncthreads();
   if (threadIdx.x < D) {
-    float mm = s_m[0];
-    for (int w = 1; w < kW; ++w) mm = fmaxf(mm, s_m[w]);
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) mm = fmaxf(mm, s_l[w] == 0.0f ? -INFINITY : s_m[w]);
     float ll = 0.0f, y = 0.0f;
+#pragma unroll
     for (int w = 0; w < kW; ++w) {
-      if (s_l[w] == 0.0f) continue;
-      const float f = exp2_approx(s_m[w] - mm);
+      const float f = s_l[w] == 0.0f ? 0.0f : s_l[w] == s_l[w] ? exp2_approx(s_m[w] - mm) : 1.0f;
       ll += f * s_l[w];
       y += f * s_a[w][threadIdx.x];
     }
-    const int token = row / p.group;
-    p.out[(size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D + threadIdx.x] =
-        __float2half_rn(ll == 0.0f ? 0.0f : y / ll);
+    out[threadIdx.x] = __float2half_rn(ll == 0.0f ? 0.0f : y / ll);
   }
 }
 
@@ -661,7 +689,8 @@ int launch(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
   if (rc != LIGER_OK || WHOLE) return rc;
   // launched while the first kernel runs; waits for it on the device
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(pl.records, pl.live);
+  const int rows_cta = pl.records * pl.live <= 4 * pl.workers ? 1 : 8;
+  cfg.gridDim = dim3(pl.records, (pl.live + rows_cta - 1) / rows_cta);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -669,7 +698,7 @@ int launch(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  LIGER_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_join_kernel<D, NT>, ap));
+  LIGER_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_join_kernel<D, NT>, ap, rows_cta));
   return LIGER_OK;
 }
 

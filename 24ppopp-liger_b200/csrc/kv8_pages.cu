@@ -248,9 +248,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_compact_plan_kernel(const Pa
   }
 }
 
-// Copies the planned pages, 16 KB of one page, layer and array at a time.
+// Copies the planned pages, 32 KB of one page, layer and array at a time.
 __device__ __forceinline__ void move_pages(const PagesParams& p) {
-  constexpr int kPiece = kMoveThreads * 4 * 16;
+  constexpr int kU = 8;
+  constexpr int kPiece = kMoveThreads * kU * 16;
   const int moves = *p.n_moves;
   const long long pieces = (long long)((p.page_codes + kPiece - 1) / kPiece);
   const long long per_page = 2 * pieces, all = (long long)moves * p.layers * per_page;
@@ -265,12 +266,12 @@ __device__ __forceinline__ void move_pages(const PagesParams& p) {
     const uint4* s = reinterpret_cast<const uint4*>(codes + from * p.page_codes + at);
     uint4* d = reinterpret_cast<uint4*>(codes + to * p.page_codes + at);
     const int left = (int)((p.page_codes - at < (size_t)kPiece ? p.page_codes - at : (size_t)kPiece) / 16);
-    uint4 x[4];
+    uint4 x[kU];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kU; ++i)
       if ((int)threadIdx.x + i * kMoveThreads < left) x[i] = __ldcs(s + threadIdx.x + i * kMoveThreads);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kU; ++i)
       if ((int)threadIdx.x + i * kMoveThreads < left) __stcs(d + threadIdx.x + i * kMoveThreads, x[i]);
     if (at == 0) {
       float* sc = is_v ? p.vs : p.ks;
