@@ -21,7 +21,7 @@
 // goes to scratch and a second, small kernel joins the parts; it is launched early and waits for the first.  Short calls with few
 // tiles give each tile to the four warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
 // stages of its own with 16-byte asynchronous copies.
-#include "kv8.cuh"
+#include "kv8_attention.cuh"
 
 namespace liger {
 namespace {
@@ -31,26 +31,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kStep = 16;            // keys of a step
 constexpr int kTileCost = 4;         // what it costs to begin a tile, in steps
 constexpr int kMinPlaces = 8;        // places that are worth a warp
+constexpr int kFewRows = 24;         // rows a key head up to which this kernel is taken
 constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttnParams {
-  Kv8Layer c;
-  Kv8Entries e;
-  const __half* q;
-  __half* out;
-  const int* kv_lens;
-  long long q_batch_stride, q_token_stride, q_head_stride;
-  int heads, group, max_kv_len, ldo, causal;
-  float scale_log2;
-  int tiles;         // most tiles of an entry
-  // shares
-  int workers;       // warps of the launch
-  int by_tile;       // 1: records are numbered by entry and tile, 0: by the worker that began the tile
-  int2* records;     // a tile that is split: the workers that have its first and its last part (else x = -1)
-  int4* tile_of;     // by worker only: the entry, tile of that record
-  float* parts;      // [2 * workers] partial results
-  DeviceStatus* status;
-};
 
 template <int D, int NT>
 struct Cfg {
@@ -75,105 +57,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// An entry of the call with everything checked: n new tokens (rows row0 ..), len keys.  A bad length or slot gives len 0.
-struct Entry {
-  int n, row0, len, slot;
-};
-__device__ __forceinline__ Entry load_entry(const AttnParams& p, int b, bool report) {
-  Entry e;
-  if (!kv8_rows(p.e, b, e.n, e.row0) && report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention, b, 0);
-  e.len = __ldg(p.kv_lens + b);
-  e.slot = kv8_slot(p.e, b);
-  if (e.len < 0 || e.len > p.max_kv_len || e.slot < 0 || e.slot >= p.c.slots || e.len > ((long long)p.c.max_pages << p.c.page_shift)) {
-    if (report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 1, b, (unsigned)e.len);
-    e.len = 0;
-  }
-  return e;
-}
-template <int ROWS>
-__device__ __forceinline__ int row_tiles(const AttnParams& p, const Entry& e) { return (e.n * p.group + ROWS - 1) / ROWS; }
 // an entry without keys still has rows to fill with zeros
 __device__ __forceinline__ int steps_of(const Entry& e) { return max(1, (e.len + kStep - 1) / kStep); }
 __device__ __forceinline__ int places_of(const Entry& e) { return steps_of(e) + kTileCost; }
 template <int ROWS>
-__device__ __forceinline__ long long line_of(const AttnParams& p, const Entry& e) {
+__device__ __forceinline__ long long line_of(const Kv8AttnParams& p, const Entry& e) {
   return (long long)p.c.kv_heads * row_tiles<ROWS>(p, e) * places_of(e);
-}
-
-__device__ __forceinline__ int workers_used(long long total, int workers) {
-  const long long want = (total + kMinPlaces - 1) / kMinPlaces;
-  return (int)(want < workers ? want : workers);
-}
-__device__ __forceinline__ long long share_begin(long long total, int used, int w) { return total * w / used; }
-__device__ __forceinline__ int share_of(long long total, int used, long long at) {  // the worker whose share has place `at`
-  int w = (int)(at * used / total);
-  while (share_begin(total, used, w + 1) <= at) ++w;
-  while (share_begin(total, used, w) > at) --w;
-  return w;
-}
-
-// The line's length, and for each warp of the CTA the entry in which its share begins and that entry's first place (entry -1:
-// the warp has no share).
-template <int ROWS>
-__device__ __forceinline__ void find_shares(const AttnParams& p, long long& total, int& used, int& b_out, long long& b_first) {
-  __shared__ long long s_warp[kWarps], s_first[kWarps];
-  __shared__ int s_b[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine = 0;
-  for (int b = threadIdx.x; b < p.e.batch; b += kThreads) mine += line_of<ROWS>(p, load_entry(p, b, blockIdx.x == 0));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_warp[warp] = mine;
-  if (threadIdx.x < kWarps) s_b[threadIdx.x] = -1;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += s_warp[w];
-  used = workers_used(total, p.workers);
-  __syncthreads();
-  const int w0 = blockIdx.x * kWarps;
-  if (w0 < used) {
-    const long long last = share_begin(total, used, min(w0 + kWarps, used) - 1);  // where the last of the CTA's shares begins
-    long long before = 0;
-    for (int base = 0; base < p.e.batch && before <= last; base += kThreads) {
-      const int b = base + threadIdx.x;
-      const long long v = b < p.e.batch ? line_of<ROWS>(p, load_entry(p, b, false)) : 0;
-      long long incl = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      if (lane == 31) s_warp[warp] = incl;
-      __syncthreads();
-      long long all = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) incl += s_warp[w];
-        all += s_warp[w];
-      }
-      const long long lo = before + incl - v, hi = before + incl;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w0 + w >= used) break;
-        const long long at = share_begin(total, used, w0 + w);
-        if (at >= lo && at < hi) { s_b[w] = b; s_first[w] = lo; }
-      }
-      before += all;
-      __syncthreads();
-    }
-  }
-  b_out = s_b[warp];
-  b_first = s_first[warp];
 }
 
 // 16-byte chunk `c` of key `r` of a step.  The xor spreads both ways of reading over all banks: a lane quad reads a key
@@ -185,7 +78,7 @@ __device__ __forceinline__ int stage_at(int r, int c) {
 }
 
 template <int D, int TYPE, int NT, int WHOLE>
-__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_kernel(const Kv8AttnParams p) {
   using C = Cfg<D, NT>;
   constexpr int kKk = D / 16;                     // k-steps of a score product = dim tiles of an output product
   constexpr int kStride = WHOLE ? kWarps : 1;     // the warps of a whole tile take every fourth step
@@ -208,7 +101,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_ker
     at = (long long)blockIdx.x * places_of(e);
     end = at + places_of(e);
   } else {
-    find_shares<C::kRows>(p, total, used, b, b_first);
+    __shared__ Kv8Shares<kWarps> shares;
+    find_shares<kThreads>(p, kMinPlaces, [&](const Entry& x) { return line_of<C::kRows>(p, x); }, shares);
+    total = shares.total;
+    used = shares.used;
+    b = shares.b[warp];
+    b_first = shares.first[warp];
     if (!p.by_tile && lane == 0) p.records[worker].x = -1;
     if (b < 0) return;
     at = share_begin(total, used, worker);
@@ -558,121 +456,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_ker
   }
 }
 
-constexpr int kJoinThreads = 256;
-
-// Joins the parts of the tiles that are split over several shares.  A CTA has the rows [blockIdx.y * rows_cta, ..) of a tile:
-// one row for its eight warps where there are few tiles, which are then split into many parts, else eight rows, one a warp.
-// The parts' maxima and sums are looked at first, 32 at a time, so that the accumulators are read without waiting for one another.
-template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const AttnParams p, int rows_cta) {
-  using C = Cfg<D, NT>;
-  constexpr int kW = kJoinThreads / 32, kA = D / 32;
-  __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
-  Entry e;
-  if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel
-  // every CTA waits, also one that has nothing to do: what follows on the stream counts on the first kernel's end
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.by_tile && tile >= p.c.kv_heads * row_tiles<C::kRows>(p, e)) return;
-  const int2 rec = p.records[blockIdx.x];
-  if (rec.x < 0) return;
-  if (!p.by_tile) {
-    const int4 at = p.tile_of[blockIdx.x];
-    b = at.x;
-    tile = at.y;
-    e = load_entry(p, b, false);
-  }
-  const bool shared = rows_cta == 1;
-  const int r = shared ? blockIdx.y : blockIdx.y * rows_cta + warp;
-  const int tiles = row_tiles<C::kRows>(p, e);
-  const int head = tile / tiles, row = (tile % tiles) * C::kRows + r;
-  if (r >= C::kRows || row >= e.n * p.group) return;  // the whole CTA where it shares a row
-  const int first = rec.x + (shared ? warp : 0), stride = shared ? kW : 1;
-  const int parts = rec.y >= first ? (rec.y - first) / stride + 1 : 0;
-  // the first part is its worker's last tile, the others are their workers' first
-  auto part_of = [&](int i) {
-    const int w = first + i * stride;
-    return p.parts + (size_t)(2 * w + (w == rec.x ? 1 : 0)) * C::kPart;
-  };
-  float m = -INFINITY, l = 0.0f, a[kA];
-#pragma unroll
-  for (int i = 0; i < kA; ++i) a[i] = 0.0f;
-  for (int base = 0; base < parts; base += 32) {
-    float pm = -INFINITY, pl = 0.0f;
-    if (base + lane < parts) {
-      const float* q = part_of(base + lane);
-      pm = __ldcg(q + r);
-      pl = __ldcg(q + C::kRows + r);
-    }
-    const float m_new = fmaxf(m, warp_max(pl == 0.0f ? -INFINITY : pm));
-    // a part that saw nothing has no weight; a NaN stays
-    const float f = pl == 0.0f ? 0.0f : pl == pl ? exp2_approx(pm - m_new) : 1.0f;
-    const float fa = l == 0.0f ? 0.0f : l == l ? exp2_approx(m - m_new) : 1.0f;
-    m = m_new;
-    l = l * fa + warp_sum(f * pl);
-#pragma unroll
-    for (int i = 0; i < kA; ++i) a[i] *= fa;
-    const int n = min(32, parts - base);
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const float fj = __shfl_sync(0xffffffffu, f, j);
-      const float* q = part_of(base + j) + 2 * C::kRows + r * D + lane * kA;
-      if (D == 128) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(q));
-        a[0] += v.x * fj; a[1] += v.y * fj; a[2 % kA] += v.z * fj; a[3 % kA] += v.w * fj;
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
-        a[0] += v.x * fj; a[1] += v.y * fj;
-      }
-    }
-  }
-  const int token = row / p.group;
-  __half* out = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
-  if (!shared) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (D == 128)
-      *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack_half2(a[0] * inv, a[1] * inv), pack_half2(a[2 % kA] * inv, a[3 % kA] * inv));
-    else
-      *reinterpret_cast<uint32_t*>(out + lane * 2) = pack_half2(a[0] * inv, a[1] * inv);
-    return;
-  }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-#pragma unroll
-  for (int i = 0; i < kA; ++i) s_a[warp][lane * kA + i] = a[i];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) mm = fmaxf(mm, s_l[w] == 0.0f ? -INFINITY : s_m[w]);
-    float ll = 0.0f, y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) {
-      const float f = s_l[w] == 0.0f ? 0.0f : s_l[w] == s_l[w] ? exp2_approx(s_m[w] - mm) : 1.0f;
-      ll += f * s_l[w];
-      y += f * s_a[w][threadIdx.x];
-    }
-    out[threadIdx.x] = __float2half_rn(ll == 0.0f ? 0.0f : y / ll);
-  }
-}
-
-struct Plan {
-  int nt, rows, live, tiles, whole, workers, by_tile, records;
-  size_t bytes;  // of scratch
-};
-
-// How a call is launched; a function of its sizes and the SM count alone.
-Plan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm_count) {
-  Plan p;
+Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm_count) {
+  Kv8AttnPlan p;
   const long long rows = (long long)a->q_len * (a->heads / c->kv_heads);
-  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
-  p.rows = 8 * p.nt;
+  const bool tc = rows > kFewRows && a->scale > 0.0f;
+  p.nt = tc ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
+  p.rows = tc ? 256 : 8 * p.nt;
   p.live = (int)(rows < p.rows ? rows : p.rows);
   const long long tiles = (long long)c->kv_heads * ((rows + p.rows - 1) / p.rows);
   p.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
-  const int ctas = (p.nt == 1 ? 3 : 2) * sm_count;
-  p.whole = a->max_kv_len <= 1024 && tiles * a->batch <= ctas;
-  p.workers = ctas * kWarps;
+  const int ctas = (tc ? 1 : p.nt == 1 ? 3 : 2) * sm_count;
+  p.whole = !tc && a->max_kv_len <= 1024 && tiles * a->batch <= ctas;
+  p.workers = tc ? ctas : ctas * kWarps;
   p.by_tile = tiles * a->batch <= p.workers;
   p.records = p.by_tile ? p.tiles * a->batch : p.workers;
   p.bytes = p.whole ? 0 : (size_t)p.workers * (sizeof(int2) + sizeof(int4)) + (size_t)2 * p.workers * p.rows * (c->head_dim + 2) * sizeof(float);
@@ -680,30 +475,18 @@ Plan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm
 }
 
 template <int D, int TYPE, int NT, int WHOLE>
-int launch(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
+int launch(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
   using C = Cfg<D, NT>;
   LIGER_CUDA_TRY(cudaFuncSetAttribute(kv8_attention_kernel<D, TYPE, NT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   const dim3 grid = WHOLE ? dim3(pl.tiles, ap.e.batch) : dim3(pl.workers / kWarps);
   kv8_attention_kernel<D, TYPE, NT, WHOLE><<<grid, kThreads, C::kSmem, s>>>(ap);
   int rc = check_launch("kv8_attention_kernel");
   if (rc != LIGER_OK || WHOLE) return rc;
-  // launched while the first kernel runs; waits for it on the device
-  cudaLaunchConfig_t cfg{};
-  const int rows_cta = pl.records * pl.live <= 4 * pl.workers ? 1 : 8;
-  cfg.gridDim = dim3(pl.records, (pl.live + rows_cta - 1) / rows_cta);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  LIGER_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_join_kernel<D, NT>, ap, rows_cta));
-  return LIGER_OK;
+  return launch_join<D, 8 * NT>(ap, pl, s);
 }
 
 template <int D, int TYPE>
-int launch_rows(const AttnParams& ap, const Plan& pl, cudaStream_t s) {
+int launch_rows(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
   if (pl.whole) return pl.nt == 1 ? launch<D, TYPE, 1, 1>(ap, pl, s) : pl.nt == 2 ? launch<D, TYPE, 2, 1>(ap, pl, s) : launch<D, TYPE, 3, 1>(ap, pl, s);
   return pl.nt == 1 ? launch<D, TYPE, 1, 0>(ap, pl, s) : pl.nt == 2 ? launch<D, TYPE, 2, 0>(ap, pl, s) : launch<D, TYPE, 3, 0>(ap, pl, s);
 }
@@ -756,11 +539,11 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   if (!a->scratch && plan_of(cache, a, kAssumedSms).bytes) return set_error(LIGER_ERR_INVALID, "kv8_attention: scratch is NULL");
   const DeviceInfo* dev = current_device();
   if (!dev) return LIGER_ERR_CUDA;
-  const Plan pl = plan_of(cache, a, dev->sm_count);
+  const Kv8AttnPlan pl = plan_of(cache, a, dev->sm_count);
   if (a->scratch_bytes < pl.bytes)
     return set_error(LIGER_ERR_TOO_LARGE, "kv8_attention: scratch has %zu bytes, %zu are needed", a->scratch_bytes, pl.bytes);
   if (pl.tiles == 0x7fffffff) return set_error(LIGER_ERR_UNSUPPORTED, "kv8_attention: q_len %d x heads %d is too large", a->q_len, a->heads);
-  AttnParams p{};
+  Kv8AttnParams p{};
   p.c = kv8_layer(cache, a->layer);
   p.e = Kv8Entries{a->q_offsets, a->slots, a->batch, a->q_len, a->total_tokens};
   p.q = (const __half*)a->q;
@@ -783,6 +566,7 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   p.records = (int2*)(p.tile_of + pl.workers);
   p.status = dev->status_dev;
   cudaStream_t s = (cudaStream_t)stream;
+  if (pl.nt == 0) return launch_kv8_attention_tc(p, pl, cache->head_dim, cache->type, s);
   if (cache->head_dim == 128)
     return cache->type == LIGER_KV8_INT8 ? launch_rows<128, LIGER_KV8_INT8>(p, pl, s) : launch_rows<128, LIGER_KV8_E4M3>(p, pl, s);
   return cache->type == LIGER_KV8_INT8 ? launch_rows<64, LIGER_KV8_INT8>(p, pl, s) : launch_rows<64, LIGER_KV8_E4M3>(p, pl, s);

@@ -1,0 +1,265 @@
+// What the two kernels of attention over the paged 8-bit cache share: the call as the device sees it, equal shares of all
+// sequences' work, and joining the parts of what lies across the border of two shares.
+//
+// Work is counted in places.  A tile (sequence, key head, row tile) has one for each step along its keys and a few for what it
+// costs to begin one.  All tiles' places form one line, of which each worker (a warp or a CTA) takes an equal piece, whatever
+// the sequences' lengths are.
+#pragma once
+#include "kv8.cuh"
+
+namespace liger {
+
+struct Kv8AttnParams {
+  Kv8Layer c;
+  Kv8Entries e;
+  const __half* q;
+  __half* out;
+  const int* kv_lens;
+  long long q_batch_stride, q_token_stride, q_head_stride;
+  int heads, group, max_kv_len, ldo, causal;
+  float scale_log2;
+  int tiles;         // most tiles of an entry
+  // shares
+  int workers;       // warps or CTAs that share the work
+  int by_tile;       // 1: records are numbered by entry and tile, 0: by the worker that began the tile
+  int2* records;     // a tile that is split: the workers that have its first and its last part (else x = -1)
+  int4* tile_of;     // by worker only: the entry, tile of that record
+  float* parts;      // [2 * workers] partial results
+  DeviceStatus* status;
+};
+
+
+// What a launch takes, as a function of a call's sizes and the SM count alone.
+struct Kv8AttnPlan {
+  int rows;      // rows of a tile
+  int live;      // rows of a tile that can be in use
+  int nt;        // kv8_attention_kernel's row groups; 0: kv8_attention_tc_kernel
+  int tiles;     // most tiles of an entry
+  int whole;     // kv8_attention_kernel: a CTA takes a whole tile
+  int workers, by_tile, records;
+  size_t bytes;  // of scratch
+};
+
+// kv8_attention_sm100.cu
+int launch_kv8_attention_tc(const Kv8AttnParams& p, const Kv8AttnPlan& pl, int head_dim, int type, cudaStream_t stream);
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// An entry of the call with everything checked: n new tokens (rows row0 ..), len keys.  A bad length or slot gives len 0.
+struct Entry {
+  int n, row0, len, slot;
+};
+__device__ __forceinline__ Entry load_entry(const Kv8AttnParams& p, int b, bool report) {
+  Entry e;
+  if (!kv8_rows(p.e, b, e.n, e.row0) && report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention, b, 0);
+  e.len = __ldg(p.kv_lens + b);
+  e.slot = kv8_slot(p.e, b);
+  if (e.len < 0 || e.len > p.max_kv_len || e.slot < 0 || e.slot >= p.c.slots || e.len > ((long long)p.c.max_pages << p.c.page_shift)) {
+    if (report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 1, b, (unsigned)e.len);
+    e.len = 0;
+  }
+  return e;
+}
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const Kv8AttnParams& p, const Entry& e) { return (e.n * p.group + ROWS - 1) / ROWS; }
+
+__device__ __forceinline__ int workers_used(long long total, int workers, int least) {
+  const long long want = (total + least - 1) / least;
+  return (int)(want < workers ? want : workers);
+}
+__device__ __forceinline__ long long share_begin(long long total, int used, int w) { return total * w / used; }
+__device__ __forceinline__ int share_of(long long total, int used, long long at) {  // the worker whose share has place `at`
+  int w = (int)(at * used / total);
+  while (share_begin(total, used, w + 1) <= at) ++w;
+  while (share_begin(total, used, w) > at) --w;
+  return w;
+}
+
+// Where the shares of a CTA's workers begin: entry and that entry's first place (entry -1: no share).
+template <int SHARES>
+struct Kv8Shares {
+  long long total;
+  int used;
+  int b[SHARES];
+  long long first[SHARES];
+};
+// `line` gives the places of an entry; a share has at least `least`.  Ends with a barrier of the CTA.
+template <int THREADS, int SHARES, typename Line>
+__device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, Line line, Kv8Shares<SHARES>& out) {
+  constexpr int kW = THREADS / 32;
+  __shared__ long long s_warp[kW];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long mine = 0;
+  for (int b = threadIdx.x; b < p.e.batch; b += THREADS) mine += line(load_entry(p, b, blockIdx.x == 0));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) s_warp[warp] = mine;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kW; ++w) total += s_warp[w];
+  const int used = workers_used(total, p.workers, least);
+  if (threadIdx.x == 0) { out.total = total; out.used = used; }
+  if (threadIdx.x < SHARES) out.b[threadIdx.x] = -1;
+  __syncthreads();
+  const int w0 = blockIdx.x * SHARES;
+  if (w0 < used) {
+    const long long last = share_begin(total, used, min(w0 + SHARES, used) - 1);  // where the last of the CTA's shares begins
+    long long before = 0;
+    for (int base = 0; base < p.e.batch && before <= last; base += THREADS) {
+      const int b = base + threadIdx.x;
+      const long long v = b < p.e.batch ? line(load_entry(p, b, false)) : 0;
+      long long incl = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) s_warp[warp] = incl;
+      __syncthreads();
+      long long all = 0;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        if (w < warp) incl += s_warp[w];
+        all += s_warp[w];
+      }
+      const long long lo = before + incl - v, hi = before + incl;
+#pragma unroll
+      for (int w = 0; w < SHARES; ++w) {
+        if (w0 + w >= used) break;
+        const long long at = share_begin(total, used, w0 + w);
+        if (at >= lo && at < hi) { out.b[w] = b; out.first[w] = lo; }
+      }
+      before += all;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+}
+
+constexpr int kJoinThreads = 256;
+
+// Joins the parts of the tiles that are split over several shares.  A CTA has the rows [blockIdx.y * rows_cta, ..) of a tile:
+// one row for its eight warps where there are few tiles, which are then split into many parts, else eight rows, one a warp.
+// The parts' maxima and sums are looked at first, 32 at a time, so that the accumulators are read without waiting for one another.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const Kv8AttnParams p, int rows_cta) {
+  constexpr int kPart = ROWS * (D + 2);
+  constexpr int kW = kJoinThreads / 32, kA = D / 32;
+  __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  Entry e;
+  if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel
+  // every CTA waits, also one that has nothing to do: what follows on the stream counts on the first kernel's end
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.by_tile && tile >= p.c.kv_heads * row_tiles<ROWS>(p, e)) return;
+  const int2 rec = p.records[blockIdx.x];
+  if (rec.x < 0) return;
+  if (!p.by_tile) {
+    const int4 at = p.tile_of[blockIdx.x];
+    b = at.x;
+    tile = at.y;
+    e = load_entry(p, b, false);
+  }
+  const bool shared = rows_cta == 1;
+  const int r = shared ? blockIdx.y : blockIdx.y * rows_cta + warp;
+  const int tiles = row_tiles<ROWS>(p, e);
+  const int head = tile / tiles, row = (tile % tiles) * ROWS + r;
+  if (r >= ROWS || row >= e.n * p.group) return;  // the whole CTA where it shares a row
+  const int first = rec.x + (shared ? warp : 0), stride = shared ? kW : 1;
+  const int parts = rec.y >= first ? (rec.y - first) / stride + 1 : 0;
+  // the first part is its worker's last tile, the others are their workers' first
+  auto part_of = [&](int i) {
+    const int w = first + i * stride;
+    return p.parts + (size_t)(2 * w + (w == rec.x ? 1 : 0)) * kPart;
+  };
+  float m = -INFINITY, l = 0.0f, a[kA];
+#pragma unroll
+  for (int i = 0; i < kA; ++i) a[i] = 0.0f;
+  for (int base = 0; base < parts; base += 32) {
+    float pm = -INFINITY, pl = 0.0f;
+    if (base + lane < parts) {
+      const float* q = part_of(base + lane);
+      pm = __ldcg(q + r);
+      pl = __ldcg(q + ROWS + r);
+    }
+    const float m_new = fmaxf(m, warp_max(pl == 0.0f ? -INFINITY : pm));
+    // a part that saw nothing has no weight; a NaN stays
+    const float f = pl == 0.0f ? 0.0f : pl == pl ? exp2_approx(pm - m_new) : 1.0f;
+    const float fa = l == 0.0f ? 0.0f : l == l ? exp2_approx(m - m_new) : 1.0f;
+    m = m_new;
+    l = l * fa + warp_sum(f * pl);
+#pragma unroll
+    for (int i = 0; i < kA; ++i) a[i] *= fa;
+    const int n = min(32, parts - base);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+      const float* q = part_of(base + j) + 2 * ROWS + r * D + lane * kA;
+      if (D == 128) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(q));
+        a[0] += v.x * fj; a[1] += v.y * fj; a[2 % kA] += v.z * fj; a[3 % kA] += v.w * fj;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
+        a[0] += v.x * fj; a[1] += v.y * fj;
+      }
+    }
+  }
+  const int token = row / p.group;
+  __half* out = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
+  if (!shared) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (D == 128)
+      *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack_half2(a[0] * inv, a[1] * inv), pack_half2(a[2 % kA] * inv, a[3 % kA] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out + lane * 2) = pack_half2(a[0] * inv, a[1] * inv);
+    return;
+  }
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+#pragma unroll
+  for (int i = 0; i < kA; ++i) s_a[warp][lane * kA + i] = a[i];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) mm = fmaxf(mm, s_l[w] == 0.0f ? -INFINITY : s_m[w]);
+    float ll = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      const float f = s_l[w] == 0.0f ? 0.0f : s_l[w] == s_l[w] ? exp2_approx(s_m[w] - mm) : 1.0f;
+      ll += f * s_l[w];
+      y += f * s_a[w][threadIdx.x];
+    }
+    out[threadIdx.x] = __float2half_rn(ll == 0.0f ? 0.0f : y / ll);
+  }
+}
+
+
+// Launched while the first kernel runs; waits for it on the device.
+template <int D, int ROWS>
+int launch_join(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
+  // one row a CTA where a tile can be in many parts
+  const int rows_cta = (long long)pl.tiles * ap.e.batch * 4 <= pl.workers || pl.records * pl.live <= 4096 ? 1 : 8;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(pl.records, (pl.live + rows_cta - 1) / rows_cta);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  LIGER_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_join_kernel<D, ROWS>, ap, rows_cta));
+  return LIGER_OK;
+}
+
+#endif
+
+}  // namespace liger

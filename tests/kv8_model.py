@@ -111,11 +111,11 @@ class Cache:
 
 
 def attention(cache, layer, q, n, length, slot, scale, causal):
-    """One sequence in 64 bits: q [n, heads, D] -> out [n, heads, D], and what its error bound is made of: sum p |v| and the
-    largest sum |q k| scale log2(e) of a score."""
+    """One sequence in 64 bits: q [n, heads, D] -> out [n, heads, D], and what its error bound is made of: sum p |v|, the
+    largest sum |q k| scale log2(e) of a score, the largest |v|."""
     heads, d = q.shape[1], q.shape[2]
     if not n or not length:
-        return torch.zeros((n, heads, d), dtype=torch.float64), torch.zeros((n, heads, d), dtype=torch.float64), 0.0
+        return torch.zeros((n, heads, d), dtype=torch.float64), torch.zeros((n, heads, d), dtype=torch.float64), 0.0, 0.0
     k, v = cache.values(layer, slot, length)
     g = heads // cache.kv_heads
     k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
@@ -128,15 +128,18 @@ def attention(cache, layer, q, n, length, slot, scale, causal):
     p = torch.exp(x - top.masked_fill(top == -float("inf"), 0.0))
     p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
     size = float(torch.einsum("nhd,khd->hnk", q.abs(), k.abs()).max()) * abs(scale) * 1.4427
-    return torch.einsum("hnk,khd->nhd", p, v), torch.einsum("hnk,khd->nhd", p, v.abs()), size
+    return torch.einsum("hnk,khd->nhd", p, v), torch.einsum("hnk,khd->nhd", p, v.abs()), size, float(v.abs().max())
 
 
-def attention_tolerance(want, mixed, size, d):
+def attention_tolerance(want, mixed, size, d, weights16=None):
     """fp16 result: half a step, 2^-11 relative, or 2^-25 below the normal numbers.  A score is a sum of d products in fp32
     and is off by at most d * 2^-23 * sum |q k| (each of d additions rounds or truncates); in log2 units that is a relative error
     of ln 2 times it in a weight, once above and once below the fraction.  2^-18 * sum p |v| stands for the weights' other
-    roundings: exp2 (2^-22), its argument (2^-24 times scores below 32), two fp16 parts (2^-22), the fp32 sums."""
-    return want.abs() * 2.0 ** -11 + 2.0 ** -25 + mixed * (2 * 0.6932 * d * 2.0 ** -23 * size + 2.0 ** -18)
+    roundings: exp2 (2^-22), its argument (2^-24 times scores below 32), two fp16 parts (2^-22), the fp32 sums.
+    weights16 = (keys, largest |v|): weights are rounded to one fp16 number each, 2^-11 relative, or 2^-25 below 2^-14, in units in
+    which the largest weight's share of the sum is 1 and the largest value scale so far is the unit of v."""
+    tol = want.abs() * 2.0 ** -11 + 2.0 ** -25 + mixed * (2 * 0.6932 * d * 2.0 ** -23 * size + 2.0 ** -18)
+    return tol if weights16 is None else tol + mixed * 2.0 ** -11 + weights16[0] * weights16[1] * 2.0 ** -25
 
 
 def append(cache, layer, slot, first, k, v):
