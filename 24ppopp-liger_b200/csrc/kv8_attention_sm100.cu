@@ -32,7 +32,7 @@ namespace {
 
 constexpr int kBlock = 128;         // keys of a block, rows of a half
 constexpr int kItemRows = 256;
-constexpr int kItemCost = 2;        // what it costs to begin a tile, in blocks
+constexpr int kItemCost = 1;        // what it costs to begin a tile, in blocks (fitted to the CTAs' times: 1.5)
 constexpr int kMinPlaces = 4;       // places that are worth a CTA
 constexpr int kSoftmaxWarps = 16, kCodeWarps = 8, kQueryWarps = 2;
 constexpr int kProductWarp = kSoftmaxWarps + kCodeWarps, kScaleWarp = kProductWarp + 1;
@@ -606,22 +606,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           // a thread has one 16-byte piece of every kStep-th row; row r is token r / group, head r % group
           constexpr int kStep = kQueryWarps * 32 / kQChunks;
           const int qc = qt % kQChunks;
-          int r = r0 + qt / kQChunks, token = r / p.group, hh = r - token * p.group;
+          int r = r0 + qt / kQChunks, hh = r % p.group;
+          const __half* src = base + (long long)(r / p.group) * p.q_token_stride + (long long)hh * p.q_head_stride + qc * 8;
           const int d_token = kStep / p.group, d_hh = kStep - d_token * p.group;
+          const long long d_src = d_token * p.q_token_stride + d_hh * p.q_head_stride, d_wrap = p.q_token_stride - p.group * p.q_head_stride;
           uint32_t dst = sQ + h * C::kTile + (qc >> 3) * kBox + (r & 127) * 128;
 #pragma unroll 4
           for (int i = 0; i < 128 / kStep; ++i) {
             const bool there = r < rows;  // rows that are not there are zeros
-            const __half* src = there ? base + (long long)token * p.q_token_stride + (long long)hh * p.q_head_stride + qc * 8 : p.q;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (((qc & 7) ^ (r & 7)) << 4)), "l"(src), "r"(there ? 16 : 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (((qc & 7) ^ (r & 7)) << 4)), "l"(there ? src : p.q),
+                         "r"(there ? 16 : 0)
                          : "memory");
             r += kStep;
             dst += kStep * 128;
-            token += d_token;
+            src += d_src;
             hh += d_hh;
             if (hh >= p.group) {
               hh -= p.group;
-              ++token;
+              src += d_wrap;
             }
           }
           asm volatile("cp.async.wait_all;" ::: "memory");
@@ -656,8 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
       const int s0 = w->s0, stop = h ? w->stop1 : w->stop0, all = max(w->stop0, w->stop1);
       const int rows = w->n * p.group, r = w->rt * kItemRows + r_tile;
       const int limit = r < rows ? limit_of(p, w->len, w->n, r) : 0;
-      // the first row of this warp sees least
-      const int limit_low = __reduce_min_sync(0xffffffffu, limit);
+      const int limit_low = __reduce_min_sync(0xffffffffu, limit), limit_high = __reduce_max_sync(0xffffffffu, limit);
       float m_ref = -INFINITY, l = 0.0f, ref = 1.0f;
 #pragma unroll 1
       for (int j = s0; j < stop; ++j, ++ns) {
@@ -668,18 +669,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         const float4 rf = lds128(s_ref + slot * 16);
         ref = rf.x;
         const int cut = limit - j * kBlock - cp * 64;  // this thread's columns from here on are not seen
-        // the same in both warps: nothing is hidden from a row, no page is missing, no scale is not finite
-        const bool plain = limit_low - j * kBlock >= kBlock && rf.z == 0.0f;
+        // groups of 16 columns: the first `free` are seen by all rows of the warp (none, where a page is missing or a scale is 0 or not
+        // finite), those from `shut` on by none
+        const int free = rf.z == 0.0f ? (limit_low - j * kBlock - cp * 64) >> 4 : 0;
+        const int shut = min(4, (limit_high - j * kBlock - cp * 64 + 15) >> 4);
         // the rows' largest scores, in log2 units and without the value scales; the two warps of a row tell each other
         float mx = -INFINITY;
 #pragma unroll 1
-        for (int gi = 0; gi < 4; ++gi) {
+        for (int gi = 0; gi < shut; ++gi) {
           uint32_t x[16];
           tmem_ld_32x16(s_addr + gi * 16, x);
           const float4 f = lds128(sc + gi * 16);
           float a = -INFINITY, b = -INFINITY;
           tmem_ld_wait16(x);
-          if (plain) {
+          if (gi < free) {
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
               a = fmaxf(a, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
@@ -708,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           const float off = f.y - m_safe;
           tmem_ld_wait16(x);
           float total;
-          if (plain) {
+          if (gi < free) {
             const uint64_t f2 = pack2(f.x, f.x), off2 = pack2(off, off);
             uint64_t a = 0, b = 0;
 #pragma unroll
@@ -723,6 +726,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
             }
             const float2 ab = unpack2(add2(a, b));
             total = ab.x + ab.y;
+          } else if (gi >= shut) {
+            total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pk[i] = 0;
           } else {
             const int seen = cut - gi * 16;
             total = 0.0f;
