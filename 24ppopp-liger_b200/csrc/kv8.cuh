@@ -1,6 +1,8 @@
 // The paged 8-bit key/value cache as its kernels see it: one layer's arrays, the entries (sequences) of a call, and the
 // conversions between fp16 / fp32 and the two code types.
 #pragma once
+#include <atomic>
+
 #include "runtime.h"
 
 namespace liger {
@@ -32,6 +34,42 @@ int kv8_check_tokens(const char* what, const int* q_offsets, int batch, int q_le
                      long long token_stride, long long head_stride);
 
 #ifdef __CUDACC__
+
+// Every kernel of the cache is launched while its predecessor on the stream may still run (launch_early), waits for it here
+// before it touches memory, and lets its successor be launched.  All CTAs wait, also those that have nothing to do: a successor
+// counts on a kernel's end for the end of all that came before it.
+__device__ __forceinline__ void wait_for_stream() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... Params, typename... Args>
+int launch_early(const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(LIGER_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+  }
+  return LIGER_OK;
+}
+// Allows `kernel` this much shared memory, once on each device (the call costs about 2 us); `done` is the kernel's own.
+template <typename Kernel>
+int allow_smem(Kernel kernel, size_t bytes, const DeviceInfo* dev, std::atomic<unsigned long long>& done) {
+  const unsigned long long bit = 1ull << (dev->device & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return LIGER_OK;
+  LIGER_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return LIGER_OK;
+}
 
 // New tokens of entry b: their number, and the first one's row among all tokens of the call.  False: the offsets are not a
 // run of at most q_len rows inside [0, total_tokens).

@@ -101,6 +101,7 @@ template <int D, int TYPE, int U>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendParams p) {
   constexpr int kPieces = D / 8;  // 16-byte pieces of a source row
   __shared__ uint32_t s_max[kAppendThreads / 32];
+  wait_for_stream();
   const int b = blockIdx.y;
   int n, row0;
   const bool rows_ok = kv8_rows(p.e, b, n, row0);
@@ -228,11 +229,8 @@ template <int D, int U>
 int launch_append(const AppendParams& p, int type, cudaStream_t stream) {
   const long long units = 2ll * p.c.kv_heads * p.blocks, per = kAppendThreads / p.unit;
   const dim3 grid((unsigned)((units + per - 1) / per), p.e.batch);
-  if (type == LIGER_KV8_INT8)
-    kv8_append_kernel<D, LIGER_KV8_INT8, U><<<grid, kAppendThreads, 0, stream>>>(p);
-  else
-    kv8_append_kernel<D, LIGER_KV8_E4M3, U><<<grid, kAppendThreads, 0, stream>>>(p);
-  return check_launch("kv8_append_kernel");
+  return launch_early("kv8_append_kernel", type == LIGER_KV8_INT8 ? kv8_append_kernel<D, LIGER_KV8_INT8, U> : kv8_append_kernel<D, LIGER_KV8_E4M3, U>,
+                      grid, kAppendThreads, 0, stream, p);
 }
 
 }  // namespace

@@ -19,27 +19,29 @@
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
 // are; warps never wait for one another.  Where a share begins or ends inside a tile the partial (maximum, sum, accumulator)
 // goes to scratch and a second, small kernel joins the parts; it is launched early and waits for the first.  Short calls with few
-// tiles give each tile to the four warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
+// tiles give each tile to the eight warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
 // stages of its own with 16-byte asynchronous copies.
 #include "kv8_attention.cuh"
 
 namespace liger {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarps = 4;            // of a CTA whose warps have shares of their own
+constexpr int kWholeWarps = 8;       // of a CTA that has a whole tile
 constexpr int kStep = 16;            // keys of a step
 constexpr int kTileCost = 4;         // what it costs to begin a tile, in steps
 constexpr int kMinPlaces = 8;        // places that are worth a warp
 constexpr int kFewRows = 24;         // rows a key head up to which this kernel is taken
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, int NT>
+template <int D, int NT, int WHOLE>
 struct Cfg {
+  static constexpr int kWarps = WHOLE ? kWholeWarps : liger::kWarps;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kCtas = NT == 1 ? 3 : 2;                      // resident per SM
+  static constexpr int kCtas = WHOLE ? 1 : NT == 1 ? 3 : 2;          // resident per SM
   static constexpr int kStage = 2 * kStep * D;                       // K and V of a step
-  static constexpr int kStages = (NT == 1 ? 4 : 6) * (128 / D);
+  static constexpr int kStages = (NT == 1 || WHOLE ? 4 : 6) * (128 / D);
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kMerge = kWarps * kRows * (D + 4) * 4;        // accumulators of a CTA's warps, in the place of the rings
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
@@ -78,16 +80,17 @@ __device__ __forceinline__ int stage_at(int r, int c) {
 }
 
 template <int D, int TYPE, int NT, int WHOLE>
-__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) kv8_attention_kernel(const Kv8AttnParams p) {
-  using C = Cfg<D, NT>;
+__global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>::kCtas) kv8_attention_kernel(const Kv8AttnParams p) {
+  using C = Cfg<D, NT, WHOLE>;
+  constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kKk = D / 16;                     // k-steps of a score product = dim tiles of an output product
-  constexpr int kStride = WHOLE ? kWarps : 1;     // the warps of a whole tile take every fourth step
+  constexpr int kStride = WHOLE ? kWarps : 1;     // the warps of a whole tile take every eighth step
   extern __shared__ __align__(128) uint8_t smem_kv8[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_kv8 + warp * C::kStages * C::kStage;
   const uint32_t ring_u = smem_u32(ring);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_for_stream();
 
   // the places [at, end) of the line, beginning in entry b whose places start at b_first
   long long total = 0, at = 0, end = 0, b_first = 0;
@@ -466,7 +469,7 @@ Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a,
   const long long tiles = (long long)c->kv_heads * ((rows + p.rows - 1) / p.rows);
   p.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
   const int ctas = (tc ? 1 : p.nt == 1 ? 3 : 2) * sm_count;
-  p.whole = !tc && a->max_kv_len <= 1024 && tiles * a->batch <= ctas;
+  p.whole = !tc && a->max_kv_len <= 1024 && tiles * a->batch <= sm_count;
   p.workers = tc ? ctas : ctas * kWarps;
   p.by_tile = tiles * a->batch <= p.workers;
   p.records = p.by_tile ? p.tiles * a->batch : p.workers;
@@ -475,20 +478,20 @@ Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a,
 }
 
 template <int D, int TYPE, int NT, int WHOLE>
-int launch(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
-  using C = Cfg<D, NT>;
-  LIGER_CUDA_TRY(cudaFuncSetAttribute(kv8_attention_kernel<D, TYPE, NT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+int launch(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
+  using C = Cfg<D, NT, WHOLE>;
+  static std::atomic<unsigned long long> allowed{0};
+  int rc = allow_smem(kv8_attention_kernel<D, TYPE, NT, WHOLE>, C::kSmem, dev, allowed);
+  if (rc != LIGER_OK) return rc;
   const dim3 grid = WHOLE ? dim3(pl.tiles, ap.e.batch) : dim3(pl.workers / kWarps);
-  kv8_attention_kernel<D, TYPE, NT, WHOLE><<<grid, kThreads, C::kSmem, s>>>(ap);
-  int rc = check_launch("kv8_attention_kernel");
-  if (rc != LIGER_OK || WHOLE) return rc;
-  return launch_join<D, 8 * NT>(ap, pl, s);
+  rc = launch_early("kv8_attention_kernel", kv8_attention_kernel<D, TYPE, NT, WHOLE>, grid, C::kThreads, C::kSmem, s, ap);
+  return rc != LIGER_OK || WHOLE ? rc : launch_join<D, 8 * NT>(ap, pl, s);
 }
 
 template <int D, int TYPE>
-int launch_rows(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
-  if (pl.whole) return pl.nt == 1 ? launch<D, TYPE, 1, 1>(ap, pl, s) : pl.nt == 2 ? launch<D, TYPE, 2, 1>(ap, pl, s) : launch<D, TYPE, 3, 1>(ap, pl, s);
-  return pl.nt == 1 ? launch<D, TYPE, 1, 0>(ap, pl, s) : pl.nt == 2 ? launch<D, TYPE, 2, 0>(ap, pl, s) : launch<D, TYPE, 3, 0>(ap, pl, s);
+int launch_rows(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
+  if (pl.whole) return pl.nt == 1 ? launch<D, TYPE, 1, 1>(ap, pl, dev, s) : pl.nt == 2 ? launch<D, TYPE, 2, 1>(ap, pl, dev, s) : launch<D, TYPE, 3, 1>(ap, pl, dev, s);
+  return pl.nt == 1 ? launch<D, TYPE, 1, 0>(ap, pl, dev, s) : pl.nt == 2 ? launch<D, TYPE, 2, 0>(ap, pl, dev, s) : launch<D, TYPE, 3, 0>(ap, pl, dev, s);
 }
 
 int check_args(const liger_kv8_cache* c, const liger_kv8_attention_args* a) {
@@ -537,8 +540,8 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   if (((uintptr_t)a->kv_lens | (uintptr_t)a->slots) & 3u)
     return set_error(LIGER_ERR_INVALID, "kv8_attention: kv_lens and slots must be 4-byte aligned");
   if (!a->scratch && plan_of(cache, a, kAssumedSms).bytes) return set_error(LIGER_ERR_INVALID, "kv8_attention: scratch is NULL");
-  const DeviceInfo* dev = current_device();
-  if (!dev) return LIGER_ERR_CUDA;
+  const DeviceInfo* dev = nullptr;
+  if ((rc = require_sm100(&dev)) != LIGER_OK) return rc;
   const Kv8AttnPlan pl = plan_of(cache, a, dev->sm_count);
   if (a->scratch_bytes < pl.bytes)
     return set_error(LIGER_ERR_TOO_LARGE, "kv8_attention: scratch has %zu bytes, %zu are needed", a->scratch_bytes, pl.bytes);
@@ -566,8 +569,8 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   p.records = (int2*)(p.tile_of + pl.workers);
   p.status = dev->status_dev;
   cudaStream_t s = (cudaStream_t)stream;
-  if (pl.nt == 0) return launch_kv8_attention_tc(p, pl, cache->head_dim, cache->type, s);
+  if (pl.nt == 0) return launch_kv8_attention_tc(p, pl, cache->head_dim, cache->type, dev, s);
   if (cache->head_dim == 128)
-    return cache->type == LIGER_KV8_INT8 ? launch_rows<128, LIGER_KV8_INT8>(p, pl, s) : launch_rows<128, LIGER_KV8_E4M3>(p, pl, s);
-  return cache->type == LIGER_KV8_INT8 ? launch_rows<64, LIGER_KV8_INT8>(p, pl, s) : launch_rows<64, LIGER_KV8_E4M3>(p, pl, s);
+    return cache->type == LIGER_KV8_INT8 ? launch_rows<128, LIGER_KV8_INT8>(p, pl, dev, s) : launch_rows<128, LIGER_KV8_E4M3>(p, pl, dev, s);
+  return cache->type == LIGER_KV8_INT8 ? launch_rows<64, LIGER_KV8_INT8>(p, pl, dev, s) : launch_rows<64, LIGER_KV8_E4M3>(p, pl, dev, s);
 }

@@ -41,7 +41,7 @@ struct Kv8AttnPlan {
 };
 
 // kv8_attention_sm100.cu
-int launch_kv8_attention_tc(const Kv8AttnParams& p, const Kv8AttnPlan& pl, int head_dim, int type, cudaStream_t stream);
+int launch_kv8_attention_tc(const Kv8AttnParams& p, const Kv8AttnPlan& pl, int head_dim, int type, const DeviceInfo* dev, cudaStream_t stream);
 
 #ifdef __CUDACC__
 
@@ -156,9 +156,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
   Entry e;
-  if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel
-  // every CTA waits, also one that has nothing to do: what follows on the stream counts on the first kernel's end
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel, which has waited for what does
+  wait_for_stream();
   if (p.by_tile && tile >= p.c.kv_heads * row_tiles<ROWS>(p, e)) return;
   const int2 rec = p.records[blockIdx.x];
   if (rec.x < 0) return;
@@ -242,22 +241,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
 }
 
 
-// Launched while the first kernel runs; waits for it on the device.
 template <int D, int ROWS>
 int launch_join(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
   // one row a CTA where a tile can be in many parts
   const int rows_cta = (long long)pl.tiles * ap.e.batch * 4 <= pl.workers || pl.records * pl.live <= 4096 ? 1 : 8;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(pl.records, (pl.live + rows_cta - 1) / rows_cta);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  LIGER_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_join_kernel<D, ROWS>, ap, rows_cta));
-  return LIGER_OK;
+  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS>, dim3(pl.records, (pl.live + rows_cta - 1) / rows_cta),
+                      kJoinThreads, 0, s, ap, rows_cta);
 }
 
 #endif

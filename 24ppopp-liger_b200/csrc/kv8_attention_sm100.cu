@@ -318,7 +318,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
   __shared__ Segment segments[kTiles];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       bar_init(q_full + i * 8, kQueryWarps);
@@ -347,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
     tmem_relinquish();
   }
   tc_fence_before();
+  wait_for_stream();
   find_shares<kThreads>(p, kMinPlaces, [&](const Entry& x) { return (long long)p.c.kv_heads * head_places(p, x); }, shares);
   tc_fence_after();
   uint32_t tmem;
@@ -835,21 +835,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
 }
 
 template <int D, int TYPE>
-int launch(const Kv8AttnParams& p, const Kv8AttnPlan& pl, cudaStream_t s) {
-  LIGER_CUDA_TRY(cudaFuncSetAttribute(kv8_attention_tc_kernel<D, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
-  kv8_attention_tc_kernel<D, TYPE><<<pl.workers, kThreads, Cfg<D>::kSmem, s>>>(p);
-  const int rc = check_launch("kv8_attention_tc_kernel");
+int launch(const Kv8AttnParams& p, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
+  static std::atomic<unsigned long long> allowed{0};
+  int rc = allow_smem(kv8_attention_tc_kernel<D, TYPE>, Cfg<D>::kSmem, dev, allowed);
+  if (rc != LIGER_OK) return rc;
+  rc = launch_early("kv8_attention_tc_kernel", kv8_attention_tc_kernel<D, TYPE>, dim3(pl.workers), kThreads, Cfg<D>::kSmem, s, p);
   return rc != LIGER_OK ? rc : launch_join<D, kItemRows>(p, pl, s);
 }
 
 }  // namespace
 
-int launch_kv8_attention_tc(const Kv8AttnParams& p, const Kv8AttnPlan& pl, int head_dim, int type, cudaStream_t s) {
-  const DeviceInfo* dev = nullptr;
-  const int rc = require_sm100(&dev);
-  if (rc != LIGER_OK) return rc;
-  if (head_dim == 128) return type == LIGER_KV8_INT8 ? launch<128, LIGER_KV8_INT8>(p, pl, s) : launch<128, LIGER_KV8_E4M3>(p, pl, s);
-  return type == LIGER_KV8_INT8 ? launch<64, LIGER_KV8_INT8>(p, pl, s) : launch<64, LIGER_KV8_E4M3>(p, pl, s);
+int launch_kv8_attention_tc(const Kv8AttnParams& p, const Kv8AttnPlan& pl, int head_dim, int type, const DeviceInfo* dev, cudaStream_t s) {
+  if (head_dim == 128) return type == LIGER_KV8_INT8 ? launch<128, LIGER_KV8_INT8>(p, pl, dev, s) : launch<128, LIGER_KV8_E4M3>(p, pl, dev, s);
+  return type == LIGER_KV8_INT8 ? launch<64, LIGER_KV8_INT8>(p, pl, dev, s) : launch<64, LIGER_KV8_E4M3>(p, pl, dev, s);
 }
 
 }  // namespace liger

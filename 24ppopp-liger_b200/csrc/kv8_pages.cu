@@ -12,7 +12,11 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMoveThreads = 256;
+constexpr int kMovePiece = kMoveThreads * 8 * 16;
 constexpr int kNobody = 0x7fffffff;
+constexpr int kOwnersShared = 8192;   // slots or pages up to which the owners of a call's numbers are kept in shared memory
+constexpr int kFreeShared = 2048;     // free pages handed out that are kept there
+constexpr int kLook = 8;              // reference counts a thread looks at in a round
 
 struct PagesParams {
   uint8_t *k, *v;
@@ -74,137 +78,182 @@ __device__ __forceinline__ T block_prefix(T v, T& total, T* s_warp) {
   return before + incl - v;
 }
 
-// The first `wanted` free pages (all, if there are fewer), lowest number first, into free_list; returns how many.
-__device__ int list_free(const PagesParams& p, int wanted, int* s_warp) {
+// What a planning CTA keeps in shared memory; the same arrays lie in the workspace where they do not fit.
+struct PlanShared {
+  int warp[32];
+  long long wide[32];
+  int owner[kOwnersShared];
+  int free_list[kFreeShared];
+};
+
+// Marks the first entry that names each number of `named` inside [0, limit).
+__device__ __forceinline__ void mark_owners(const int* named, int n, int limit, int* owner) {
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int x = named[i];
+    if (x >= 0 && x < limit) owner[x] = kNobody;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int x = named[i];
+    if (x >= 0 && x < limit) atomicMin(owner + x, i);
+  }
+  __syncthreads();
+}
+
+// The first `wanted` free pages (all, if there are fewer), lowest number first, into the workspace and, those that fit, into
+// shared memory; returns how many.
+__device__ int list_free(const PagesParams& p, int wanted, PlanShared& s) {
   int found = 0;
-  for (int base = 0; base < p.num_pages && found < wanted; base += kPlanThreads * 4) {
-    const int at = base + (int)threadIdx.x * 4;
-    int f[4], c = 0, total;
+  for (int base = 0; base < p.num_pages && found < wanted; base += kPlanThreads * kLook) {
+    const int at = base + (int)threadIdx.x * kLook;
+    unsigned free = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = at + i < p.num_pages && p.refs[at + i] == 0;
-      c += f[i];
-    }
-    int rank = found + block_prefix(c, total, s_warp);
+    for (int i = 0; i < kLook; ++i) free |= (unsigned)(at + i < p.num_pages && p.refs[at + i] == 0) << i;
+    int total, rank = found + block_prefix(__popc(free), total, s.warp);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f[i]) p.free_list[rank++] = at + i;
+    for (int i = 0; i < kLook; ++i)
+      if (free >> i & 1u) {
+        p.free_list[rank] = at + i;
+        if (rank < kFreeShared) s.free_list[rank] = at + i;
+        ++rank;
+      }
     found += total;
   }
+  __syncthreads();
   return found;
 }
 
-// Marks in `owner` the first entry that names each number of `named` inside [0, limit).
-__device__ void mark_owners(const PagesParams& p, const int* named, int limit) {
-  for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
-    const int x = named[i];
-    if (x >= 0 && x < limit) p.owner[x] = kNobody;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
-    const int x = named[i];
-    if (x >= 0 && x < limit) atomicMin(p.owner + x, i);
-  }
-  __syncthreads();
-}
-
-// Hands out pages: first[i] / many[i] have how many pages entry i wants (many[i] = -1: refused already).  Entries whose pages
-// end behind the last free one are refused.  Returns the number of pages handed out.
-__device__ int hand_out(const PagesParams& p, int* s_warp) {
-  __shared__ long long s_wide[32];
+// Hands out pages.  `want(i)` gives how many entry i wants (-1: refused already), `got(i, first, n)` is told where its pages begin in
+// the list and how many they are (-1: refused).  Entries whose pages end behind the last free one are refused.  Returns the
+// number of pages handed out.  Up to 1024 entries stay in their threads' registers.
+template <typename Want, typename Got>
+__device__ int hand_out(const PagesParams& p, PlanShared& s, Want want, Got got) {
   const long long most = (long long)p.num_pages + 1;  // more than there are: refused, whatever it is exactly
   long long ends = 0;
+  int first = 0, many = -1;
   for (int base = 0; base < p.n; base += kPlanThreads) {
     const int i = base + threadIdx.x;
+    many = i < p.n ? want(i) : -1;
     long long total;
-    const long long at = ends + block_prefix<long long>(i < p.n ? max(0, p.many[i]) : 0, total, s_wide);
-    if (i < p.n) p.first[i] = (int)min(at, most);
+    first = (int)min(ends + block_prefix<long long>(max(0, many), total, s.wide), most);
     ends += total;
+    if (p.n > kPlanThreads && i < p.n) {
+      p.first[i] = first;
+      p.many[i] = many;
+    }
   }
-  const int found = list_free(p, (int)min(ends, (long long)p.num_pages), s_warp);
-  __syncthreads();
+  const int found = list_free(p, (int)min(ends, (long long)p.num_pages), s);
   int given = 0;
   for (int base = 0; base < p.n; base += kPlanThreads) {
     const int i = base + threadIdx.x;
-    int mine = 0;
-    if (i < p.n && p.many[i] > 0) {
-      if (p.many[i] > found - p.first[i]) p.many[i] = -1;
-      else mine = p.many[i];
+    if (p.n > kPlanThreads && i < p.n) {
+      first = p.first[i];
+      many = p.many[i];
     }
+    if (i >= p.n) many = -1;
+    if (many > 0 && many > found - first) many = -1;
     int total;
-    block_prefix(mine, total, s_warp);
+    block_prefix(max(0, many), total, s.warp);
     given += total;
+    if (i < p.n) {
+      if (p.done) p.done[i] = many >= 0;
+      got(i, first, many);
+    }
   }
-  for (int i = threadIdx.x; i < p.n; i += kPlanThreads)
-    if (p.done) p.done[i] = p.many[i] >= 0;
   return given;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) kv8_reserve_plan_kernel(const PagesParams p) {
-  __shared__ int s_warp[32];
-  mark_owners(p, p.dst, p.slots);
-  for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
-    const int slot = p.dst[i], len = p.lens[i];
-    int want = -1;
-    if (slot < 0 || slot >= p.slots || len < 0) {
-      report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages, i, (unsigned)slot);
-    } else if (p.owner[slot] == i) {
-      const int need = len / p.page_size + (len % p.page_size != 0);
-      if (need <= p.max_pages) want = max(0, need - max(0, p.count[slot]));
-    }
-    p.many[i] = want;
-  }
-  __syncthreads();
-  hand_out(p, s_warp);
-  if (threadIdx.x == 0) *p.n_moves = 0;
+__device__ __forceinline__ int* owners_of(const PagesParams& p, PlanShared& s, int limit) { return limit <= kOwnersShared ? s.owner : p.owner; }
+__device__ __forceinline__ int free_page(const PagesParams& p, const PlanShared& s, int i) { return i < kFreeShared ? s.free_list[i] : p.free_list[i]; }
+
+// here = 1: the entries' table rows are written by this CTA, else left to kv8_reserve_kernel
+__global__ void __launch_bounds__(kPlanThreads) kv8_reserve_plan_kernel(const PagesParams p, int here) {
+  extern __shared__ __align__(16) uint8_t smem_plan[];
+  PlanShared& s = *reinterpret_cast<PlanShared*>(smem_plan);
+  wait_for_stream();
+  int* owner = owners_of(p, s, p.slots);
+  mark_owners(p.dst, p.n, p.slots, owner);
+  hand_out(
+      p, s,
+      [&](int i) {
+        const int slot = p.dst[i], len = p.lens[i];
+        if (slot < 0 || slot >= p.slots || len < 0) {
+          report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages, i, (unsigned)slot);
+          return -1;
+        }
+        const int need = len / p.page_size + (len % p.page_size != 0);
+        return owner[slot] == i && need <= p.max_pages ? max(0, need - max(0, p.count[slot])) : -1;
+      },
+      [&](int i, int first, int many) {
+        if (here && many > 0) {
+          const int slot = p.dst[i], had = max(0, p.count[slot]);
+          int* row = p.table + (size_t)slot * p.max_pages + had;
+          for (int j = 0; j < many; ++j) {
+            const int page = free_page(p, s, first + j);
+            row[j] = page;
+            p.refs[page] = 1;
+          }
+          p.count[slot] = had + many;
+        } else if (!here) {
+          p.first[i] = first;
+          p.many[i] = many;
+        }
+      });
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv8_fork_plan_kernel(const PagesParams p) {
-  __shared__ int s_warp[32];
-  mark_owners(p, p.dst, p.slots);
-  for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
-    const int src = p.src[i], dst = p.dst[i], len = p.lens[i];
-    int want = -1;
-    if (src < 0 || src >= p.slots || dst < 0 || dst >= p.slots || len < 0) {
-      report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages + 1, i, (unsigned)dst);
-    } else if (p.owner[dst] == i && src != dst && p.count[dst] == 0) {
-      const int full = len / p.page_size, part = len % p.page_size != 0;
-      if (full + part <= min(p.count[src], p.max_pages)) want = part;
-    }
-    p.many[i] = want;
-  }
-  __syncthreads();
-  const int given = hand_out(p, s_warp);
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
-    if (p.many[i] <= 0) continue;
-    const int m = p.first[i];
-    int from = p.table[(size_t)p.src[i] * p.max_pages + p.lens[i] / p.page_size];
-    if (from < 0 || from >= p.num_pages) {
-      report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages + 3, i, (unsigned)from);
-      from = p.free_list[m];  // nothing to copy
-    }
-    p.from[m] = from;
-    p.to[m] = p.free_list[m];
-  }
+  extern __shared__ __align__(16) uint8_t smem_plan[];
+  PlanShared& s = *reinterpret_cast<PlanShared*>(smem_plan);
+  wait_for_stream();
+  int* owner = owners_of(p, s, p.slots);
+  mark_owners(p.dst, p.n, p.slots, owner);
+  const int given = hand_out(
+      p, s,
+      [&](int i) {
+        const int src = p.src[i], dst = p.dst[i], len = p.lens[i];
+        if (src < 0 || src >= p.slots || dst < 0 || dst >= p.slots || len < 0) {
+          report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages + 1, i, (unsigned)dst);
+          return -1;
+        }
+        const int full = len / p.page_size, part = len % p.page_size != 0;
+        return owner[dst] == i && src != dst && p.count[dst] == 0 && full + part <= min(p.count[src], p.max_pages) ? part : -1;
+      },
+      [&](int i, int first, int many) {
+        p.first[i] = first;
+        p.many[i] = many;
+        if (many > 0) {
+          const int to = free_page(p, s, first);
+          int from = p.table[(size_t)p.src[i] * p.max_pages + p.lens[i] / p.page_size];
+          if (from < 0 || from >= p.num_pages) {
+            report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages + 3, i, (unsigned)from);
+            from = to;  // nothing to copy
+          }
+          p.from[first] = from;
+          p.to[first] = to;
+        }
+      });
   if (threadIdx.x == 0) *p.n_moves = given;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv8_copy_plan_kernel(const PagesParams p) {
+  extern __shared__ __align__(16) uint8_t smem_plan[];
+  PlanShared& sh = *reinterpret_cast<PlanShared*>(smem_plan);
   __shared__ int s_moves;
+  wait_for_stream();
   if (threadIdx.x == 0) s_moves = 0;
+  int* owner = owners_of(p, sh, p.num_pages);
   for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
     const int s = p.src[i];
-    if (s >= 0 && s < p.num_pages) p.owner[s] = kNobody;
+    if (s >= 0 && s < p.num_pages) owner[s] = kNobody;
   }
-  mark_owners(p, p.dst, p.num_pages);
+  mark_owners(p.dst, p.n, p.num_pages, owner);
   for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
     const int s = p.src[i], d = p.dst[i];
     bool ok = false;
     if (s < 0 || s >= p.num_pages || d < 0 || d >= p.num_pages) {
       report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtPages + 2, i, (unsigned)d);
     } else {
-      ok = p.owner[d] == i && (s == d || p.owner[s] == kNobody);
+      ok = owner[d] == i && (s == d || owner[s] == kNobody);
       if (ok && s != d) {
         const int m = atomicAdd(&s_moves, 1);  // the order of the moves does not matter: their targets differ
         p.from[m] = s;
@@ -219,6 +268,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_copy_plan_kernel(const Pages
 
 __global__ void __launch_bounds__(kPlanThreads) kv8_compact_plan_kernel(const PagesParams p) {
   __shared__ int s_warp[32];
+  wait_for_stream();
   int mine = 0, live, total;
   for (int i = threadIdx.x; i < p.num_pages; i += kPlanThreads) mine += p.refs[i] != 0;
   block_prefix(mine, live, s_warp);
@@ -250,8 +300,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_compact_plan_kernel(const Pa
 
 // Copies the planned pages, 32 KB of one page, layer and array at a time.
 __device__ __forceinline__ void move_pages(const PagesParams& p) {
-  constexpr int kU = 8;
-  constexpr int kPiece = kMoveThreads * kU * 16;
+  constexpr int kU = kMovePiece / (kMoveThreads * 16), kPiece = kMovePiece;
   const int moves = *p.n_moves;
   const long long pieces = (long long)((p.page_codes + kPiece - 1) / kPiece);
   const long long per_page = 2 * pieces, all = (long long)moves * p.layers * per_page;
@@ -280,9 +329,13 @@ __device__ __forceinline__ void move_pages(const PagesParams& p) {
   }
 }
 
-__global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const PagesParams p) { move_pages(p); }
+__global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const PagesParams p) {
+  wait_for_stream();
+  move_pages(p);
+}
 
 __global__ void __launch_bounds__(kMoveThreads) kv8_fork_kernel(const PagesParams p) {
+  wait_for_stream();
   const int lane = threadIdx.x & 31;
   for (int i = (blockIdx.x * kMoveThreads + threadIdx.x) >> 5; i < p.n; i += gridDim.x * kMoveThreads / 32) {
     if (p.many[i] < 0) continue;
@@ -308,6 +361,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_fork_kernel(const PagesParam
 }
 
 __global__ void __launch_bounds__(kMoveThreads) kv8_reserve_kernel(const PagesParams p) {
+  wait_for_stream();
   const int lane = threadIdx.x & 31;
   for (int i = (blockIdx.x * kMoveThreads + threadIdx.x) >> 5; i < p.n; i += gridDim.x * kMoveThreads / 32) {
     const int more = p.many[i];
@@ -325,6 +379,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_reserve_kernel(const PagesPa
 
 // One warp per entry.  Whoever takes the count frees the slot, so a slot that is named twice is freed once.
 __global__ void __launch_bounds__(kMoveThreads) kv8_free_kernel(const PagesParams p) {
+  wait_for_stream();
   const int lane = threadIdx.x & 31;
   const int i = (int)((blockIdx.x * (size_t)kMoveThreads + threadIdx.x) >> 5);
   if (i >= p.n) return;
@@ -348,6 +403,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_free_kernel(const PagesParam
 }
 
 __global__ void __launch_bounds__(kMoveThreads) kv8_compact_kernel(const PagesParams p) {
+  wait_for_stream();
   const size_t entries = (size_t)p.slots * p.max_pages;
   for (size_t i = blockIdx.x * (size_t)kMoveThreads + threadIdx.x; i < entries; i += (size_t)gridDim.x * kMoveThreads) {
     const int page = p.table[i];
@@ -406,7 +462,11 @@ int check_ints(const char* what, const int* a, const int* b, const int* c) {
   return LIGER_OK;
 }
 
-unsigned move_grid(const DeviceInfo* dev) { return (unsigned)dev->sm_count * 8; }
+// as many CTAs as there can be pieces to move, at most eight an SM
+unsigned move_grid(const DeviceInfo* dev, const PagesParams& p, long long moves) {
+  const long long pieces = (moves < 1 ? 1 : moves) * p.layers * 2 * (long long)((p.page_codes + kMovePiece - 1) / kMovePiece);
+  return (unsigned)(pieces < (long long)dev->sm_count * 8 ? pieces : (long long)dev->sm_count * 8);
+}
 
 }  // namespace
 }  // namespace liger
@@ -429,10 +489,12 @@ extern "C" int liger_kv8_reserve(const liger_kv8_cache* cache, const int* slots,
   p.dst = slots;
   p.lens = lens;
   p.done = done;
-  kv8_reserve_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(p);
-  if ((rc = check_launch("kv8_reserve_plan_kernel")) != LIGER_OK) return rc;
-  kv8_reserve_kernel<<<dev->sm_count, kMoveThreads, 0, (cudaStream_t)stream>>>(p);
-  return check_launch("kv8_reserve_kernel");
+  // few pages at most: the planning CTA writes them down itself (a second launch costs about 3 us; a thread writes a page in
+  // about 20 ns)
+  const int here = n <= kPlanThreads && cache->max_pages <= 256;
+  rc = launch_early("kv8_reserve_plan_kernel", kv8_reserve_plan_kernel, 1, kPlanThreads, sizeof(PlanShared), (cudaStream_t)stream, p, here);
+  if (rc != LIGER_OK || here) return rc;
+  return launch_early("kv8_reserve_kernel", kv8_reserve_kernel, (unsigned)dev->sm_count, kMoveThreads, 0, (cudaStream_t)stream, p);
 }
 
 extern "C" int liger_kv8_fork(const liger_kv8_cache* cache, const int* src, const int* dst, const int* lens, int n, int* done,
@@ -447,10 +509,8 @@ extern "C" int liger_kv8_fork(const liger_kv8_cache* cache, const int* src, cons
   p.dst = dst;
   p.lens = lens;
   p.done = done;
-  kv8_fork_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(p);
-  if ((rc = check_launch("kv8_fork_plan_kernel")) != LIGER_OK) return rc;
-  kv8_fork_kernel<<<move_grid(dev), kMoveThreads, 0, (cudaStream_t)stream>>>(p);
-  return check_launch("kv8_fork_kernel");
+  if ((rc = launch_early("kv8_fork_plan_kernel", kv8_fork_plan_kernel, 1, kPlanThreads, sizeof(PlanShared), (cudaStream_t)stream, p)) != LIGER_OK) return rc;
+  return launch_early("kv8_fork_kernel", kv8_fork_kernel, move_grid(dev, p, n), kMoveThreads, 0, (cudaStream_t)stream, p);
 }
 
 extern "C" int liger_kv8_free(const liger_kv8_cache* cache, const int* slots, int n, void* stream) {
@@ -474,8 +534,7 @@ extern "C" int liger_kv8_free(const liger_kv8_cache* cache, const int* slots, in
   p.n = n;
   p.status = dev->status_dev;
   const unsigned grid = (unsigned)(((size_t)n * 32 + kMoveThreads - 1) / kMoveThreads);
-  kv8_free_kernel<<<grid, kMoveThreads, 0, (cudaStream_t)stream>>>(p);
-  return check_launch("kv8_free_kernel");
+  return launch_early("kv8_free_kernel", kv8_free_kernel, grid, kMoveThreads, 0, (cudaStream_t)stream, p);
 }
 
 extern "C" int liger_kv8_copy(const liger_kv8_cache* cache, const int* src, const int* dst, int n, int* done, void* scratch,
@@ -489,10 +548,8 @@ extern "C" int liger_kv8_copy(const liger_kv8_cache* cache, const int* src, cons
   p.src = src;
   p.dst = dst;
   p.done = done;
-  kv8_copy_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(p);
-  if ((rc = check_launch("kv8_copy_plan_kernel")) != LIGER_OK) return rc;
-  kv8_move_kernel<<<move_grid(dev), kMoveThreads, 0, (cudaStream_t)stream>>>(p);
-  return check_launch("kv8_move_kernel");
+  if ((rc = launch_early("kv8_copy_plan_kernel", kv8_copy_plan_kernel, 1, kPlanThreads, sizeof(PlanShared), (cudaStream_t)stream, p)) != LIGER_OK) return rc;
+  return launch_early("kv8_move_kernel", kv8_move_kernel, move_grid(dev, p, n), kMoveThreads, 0, (cudaStream_t)stream, p);
 }
 
 extern "C" int liger_kv8_compact(const liger_kv8_cache* cache, int* live, int* moved_to, void* scratch, size_t scratch_bytes,
@@ -504,8 +561,6 @@ extern "C" int liger_kv8_compact(const liger_kv8_cache* cache, int* live, int* m
   if ((rc = check_ints("kv8_compact", live, moved_to, nullptr)) != LIGER_OK) return rc;
   p.live = live;
   p.moved_to = moved_to ? moved_to : p.owner;
-  kv8_compact_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(p);
-  if ((rc = check_launch("kv8_compact_plan_kernel")) != LIGER_OK) return rc;
-  kv8_compact_kernel<<<move_grid(dev), kMoveThreads, 0, (cudaStream_t)stream>>>(p);
-  return check_launch("kv8_compact_kernel");
+  if ((rc = launch_early("kv8_compact_plan_kernel", kv8_compact_plan_kernel, 1, kPlanThreads, 0, (cudaStream_t)stream, p)) != LIGER_OK) return rc;
+  return launch_early("kv8_compact_kernel", kv8_compact_kernel, move_grid(dev, p, cache->num_pages), kMoveThreads, 0, (cudaStream_t)stream, p);
 }
