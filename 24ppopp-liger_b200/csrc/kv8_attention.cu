@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
           const size_t blk = (ph << (p.c.page_shift - p.c.block_shift)) + ((key & page_mask) >> p.c.block_shift);
           ks = __ldg(p.c.ks + blk);
           vs = __ldg(p.c.vs + blk);
-          if (!(vs < INFINITY)) vs = NAN;
+          if (!(ks >= 0.0f && ks < INFINITY)) ks = NAN;
+          if (!(vs >= 0.0f && vs < INFINITY)) vs = NAN;
         }
       }
     };
@@ -485,7 +486,7 @@ int launch(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev
   if (rc != LIGER_OK) return rc;
   const dim3 grid = WHOLE ? dim3(pl.tiles, ap.e.batch) : dim3(pl.workers / kWarps);
   rc = launch_early("kv8_attention_kernel", kv8_attention_kernel<D, TYPE, NT, WHOLE>, grid, C::kThreads, C::kSmem, s, ap);
-  return rc != LIGER_OK || WHOLE ? rc : launch_join<D, 8 * NT>(ap, pl, s);
+  return rc != LIGER_OK || WHOLE ? rc : launch_join<D, 8 * NT>(ap, pl, dev, s);
 }
 
 template <int D, int TYPE>

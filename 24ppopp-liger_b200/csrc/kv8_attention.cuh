@@ -95,8 +95,10 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
   constexpr int kW = THREADS / 32;
   __shared__ long long s_warp[kW];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine = 0;
-  for (int b = threadIdx.x; b < p.e.batch; b += THREADS) mine += line(load_entry(p, b, blockIdx.x == 0));
+  // most batches fit one round, whose places stay in registers
+  const long long mine0 = threadIdx.x < p.e.batch ? line(load_entry(p, threadIdx.x, blockIdx.x == 0)) : 0;
+  long long mine = mine0;
+  for (int b = threadIdx.x + THREADS; b < p.e.batch; b += THREADS) mine += line(load_entry(p, b, blockIdx.x == 0));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) s_warp[warp] = mine;
@@ -114,7 +116,7 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
     long long before = 0;
     for (int base = 0; base < p.e.batch && before <= last; base += THREADS) {
       const int b = base + threadIdx.x;
-      const long long v = b < p.e.batch ? line(load_entry(p, b, false)) : 0;
+      const long long v = base == 0 ? mine0 : b < p.e.batch ? line(load_entry(p, b, false)) : 0;
       long long incl = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -143,16 +145,14 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
   __syncthreads();
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinRowThreads = 1024, kJoinThreads = 256;
 
-// Joins the parts of the tiles that are split over several shares.  A CTA has the rows [blockIdx.y * rows_cta, ..) of a tile:
-// one row for its eight warps where there are few tiles, which are then split into many parts, else eight rows, one a warp.
-// The parts' maxima and sums are looked at first, 32 at a time, so that the accumulators are read without waiting for one another.
-template <int D, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const Kv8AttnParams p, int rows_cta) {
+// Joins the parts of the tiles that are split over several shares.  SHARED: a CTA has one row of a tile, whose parts its 32 warps
+// take in turn; else a warp has a row and takes all its parts.  Maxima, sums and accumulators of eight parts are fetched at once.
+template <int D, int ROWS, int SHARED>
+__global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_attention_join_kernel(const Kv8AttnParams p) {
   constexpr int kPart = ROWS * (D + 2);
-  constexpr int kW = kJoinThreads / 32, kA = D / 32;
-  __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
+  constexpr int kW = (SHARED ? kJoinRowThreads : kJoinThreads) / 32, kA = D / 32, kBatch = 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
   Entry e;
@@ -167,53 +167,59 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
     tile = at.y;
     e = load_entry(p, b, false);
   }
-  const bool shared = rows_cta == 1;
-  const int r = shared ? blockIdx.y : blockIdx.y * rows_cta + warp;
+  const int r = SHARED ? blockIdx.y : blockIdx.y * kW + warp;
   const int tiles = row_tiles<ROWS>(p, e);
   const int head = tile / tiles, row = (tile % tiles) * ROWS + r;
   if (r >= ROWS || row >= e.n * p.group) return;  // the whole CTA where it shares a row
-  const int first = rec.x + (shared ? warp : 0), stride = shared ? kW : 1;
-  const int parts = rec.y >= first ? (rec.y - first) / stride + 1 : 0;
-  // the first part is its worker's last tile, the others are their workers' first
-  auto part_of = [&](int i) {
-    const int w = first + i * stride;
-    return p.parts + (size_t)(2 * w + (w == rec.x ? 1 : 0)) * kPart;
-  };
+  const int first = rec.x + (SHARED ? warp : 0);
+  constexpr int kStride = SHARED ? kW : 1;
   float m = -INFINITY, l = 0.0f, a[kA];
 #pragma unroll
   for (int i = 0; i < kA; ++i) a[i] = 0.0f;
-  for (int base = 0; base < parts; base += 32) {
-    float pm = -INFINITY, pl = 0.0f;
-    if (base + lane < parts) {
-      const float* q = part_of(base + lane);
-      pm = __ldcg(q + r);
-      pl = __ldcg(q + ROWS + r);
-    }
-    const float m_new = fmaxf(m, warp_max(pl == 0.0f ? -INFINITY : pm));
-    // a part that saw nothing has no weight; a NaN stays
-    const float f = pl == 0.0f ? 0.0f : pl == pl ? exp2_approx(pm - m_new) : 1.0f;
-    const float fa = l == 0.0f ? 0.0f : l == l ? exp2_approx(m - m_new) : 1.0f;
-    m = m_new;
-    l = l * fa + warp_sum(f * pl);
+  for (int w0 = first; w0 <= rec.y; w0 += kBatch * kStride) {
+    float pm[kBatch], pl[kBatch], x[kBatch][kA];
 #pragma unroll
-    for (int i = 0; i < kA; ++i) a[i] *= fa;
-    const int n = min(32, parts - base);
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const float fj = __shfl_sync(0xffffffffu, f, j);
-      const float* q = part_of(base + j) + 2 * ROWS + r * D + lane * kA;
-      if (D == 128) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(q));
-        a[0] += v.x * fj; a[1] += v.y * fj; a[2 % kA] += v.z * fj; a[3 % kA] += v.w * fj;
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
-        a[0] += v.x * fj; a[1] += v.y * fj;
+    for (int j = 0; j < kBatch; ++j) {
+      const int w = w0 + j * kStride;
+      pm[j] = -INFINITY;
+      pl[j] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kA; ++i) x[j][i] = 0.0f;
+      if (w <= rec.y) {
+        // the first part is its worker's last tile, the others are their workers' first
+        const float* q = p.parts + (size_t)(2 * w + (w == rec.x ? 1 : 0)) * kPart;
+        pm[j] = __ldcg(q + r);
+        pl[j] = __ldcg(q + ROWS + r);
+        q += 2 * ROWS + r * D + lane * kA;
+        if (D == 128) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(q));
+          x[j][0] = v.x; x[j][1] = v.y; x[j][2 % kA] = v.z; x[j][3 % kA] = v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(q));
+          x[j][0] = v.x; x[j][1] = v.y;
+        }
       }
     }
+    float m_new = m;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) m_new = fmaxf(m_new, pl[j] == 0.0f ? -INFINITY : pm[j]);
+    // what saw nothing has no weight; a NaN stays
+    const float fa = l == 0.0f ? 0.0f : l == l ? exp2_approx(m - m_new) : 1.0f;
+    l *= fa;
+#pragma unroll
+    for (int i = 0; i < kA; ++i) a[i] *= fa;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const float f = pl[j] == 0.0f ? 0.0f : pl[j] == pl[j] ? exp2_approx(pm[j] - m_new) : 1.0f;
+      l = fmaf(f, pl[j], l);
+#pragma unroll
+      for (int i = 0; i < kA; ++i) a[i] = fmaf(f, x[j][i], a[i]);
+    }
+    m = m_new;
   }
   const int token = row / p.group;
   __half* out = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
-  if (!shared) {
+  if (!SHARED) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (D == 128)
       *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack_half2(a[0] * inv, a[1] * inv), pack_half2(a[2 % kA] * inv, a[3 % kA] * inv));
@@ -221,6 +227,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
       *reinterpret_cast<uint32_t*>(out + lane * 2) = pack_half2(a[0] * inv, a[1] * inv);
     return;
   }
+  __shared__ float s_m[kW], s_l[kW], s_a[kW][D];
   if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
 #pragma unroll
   for (int i = 0; i < kA; ++i) s_a[warp][lane * kA + i] = a[i];
@@ -240,13 +247,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(const 
   }
 }
 
-
+// Few tiles are split into many parts each: a CTA for each of their rows.
 template <int D, int ROWS>
-int launch_join(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, cudaStream_t s) {
-  // one row a CTA where a tile can be in many parts
-  const int rows_cta = (long long)pl.tiles * ap.e.batch * 4 <= pl.workers || pl.records * pl.live <= 4096 ? 1 : 8;
-  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS>, dim3(pl.records, (pl.live + rows_cta - 1) / rows_cta),
-                      kJoinThreads, 0, s, ap, rows_cta);
+int launch_join(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
+  if ((long long)pl.records * pl.live <= 2 * dev->sm_count)
+    return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 1>, dim3(pl.records, pl.live), kJoinRowThreads, 0, s, ap);
+  constexpr int kRows = kJoinThreads / 32;
+  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 0>, dim3(pl.records, (pl.live + kRows - 1) / kRows),
+                      kJoinThreads, 0, s, ap);
 }
 
 #endif

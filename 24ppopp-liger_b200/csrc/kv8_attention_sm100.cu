@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           // a slot is free when K's stage is: by then both halves are past the block before the last
           if (!bar_wait(k_empty + (g & 1u) * 8, ((g >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
           // scales of the block's eight groups: lanes 0 .. 7
-          const float mine = scale_now < INFINITY ? scale_now : NAN;
+          const float mine = scale_now >= 0.0f && scale_now < INFINITY ? scale_now : NAN;
           const float vs = __shfl_sync(0xffffffffu, mine, (lane & 7) + 8);
           const bool use = lane < 8 && page_now >= 0 && vs > 0.0f;
           const float top = warp_max(use ? vs : 0.0f);
@@ -840,7 +840,7 @@ int launch(const Kv8AttnParams& p, const Kv8AttnPlan& pl, const DeviceInfo* dev,
   int rc = allow_smem(kv8_attention_tc_kernel<D, TYPE>, Cfg<D>::kSmem, dev, allowed);
   if (rc != LIGER_OK) return rc;
   rc = launch_early("kv8_attention_tc_kernel", kv8_attention_tc_kernel<D, TYPE>, dim3(pl.workers), kThreads, Cfg<D>::kSmem, s, p);
-  return rc != LIGER_OK ? rc : launch_join<D, kItemRows>(p, pl, s);
+  return rc != LIGER_OK ? rc : launch_join<D, kItemRows>(p, pl, dev, s);
 }
 
 }  // namespace

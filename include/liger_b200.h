@@ -235,7 +235,8 @@ LIGER_API int liger_attention_decode_noalloc(const void* q, const void* k_cache,
  * What the arrays on the device say (tables, lengths, offsets) is checked by the kernels, not by the host: a page,
  * slot, position or row that does not exist is left out, and LIGER_DEV_BAD_INDEX is set in the sticky device status.
  *
- * A block into which a value that is not finite was written reads as NaN: its scale is then not finite and its codes are 0.
+ * Scales are finite and not negative.  A block into which a value that is not finite was written reads as NaN: its scale is then
+ * not finite and its codes are 0; attention takes every other scale for such a one.
  */
 #define LIGER_KV8_INT8 0 /* codes -127 .. 127 */
 #define LIGER_KV8_E4M3 1 /* fp8, 4 exponent and 3 fraction bits, largest 448 */
