@@ -93,8 +93,9 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
   wait_for_stream();
 
   // the places [at, end) of the line, beginning in entry b whose places start at b_first
-  long long total = 0, at = 0, end = 0, b_first = 0;
-  int b, used = 0;
+  long long at = 0, end = 0, b_first = 0;
+  int b;
+  Kv8Deal deal{};
   const int worker = blockIdx.x * kWarps + warp;
   Entry e;
   if (WHOLE) {
@@ -106,21 +107,21 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
   } else {
     __shared__ Kv8Shares<kWarps> shares;
     find_shares<kThreads>(p, kMinPlaces, [&](const Entry& x) { return line_of<C::kRows>(p, x); }, shares);
-    total = shares.total;
-    used = shares.used;
+    deal = shares.deal;
     b = shares.b[warp];
     b_first = shares.first[warp];
-    if (!p.by_tile && lane == 0) p.records[worker].x = -1;
+    if (!p.by_tile && lane == 0) p.records[worker].first = -1;
     if (b < 0) return;
-    at = share_begin(total, used, worker);
-    end = share_begin(total, used, worker + 1);
+    at = deal.begin(worker);
+    end = deal.begin(worker + 1);
     e = load_entry(p, b, false);
   }
   const long long share0 = at;
 
   while (at < end) {
     const int steps = steps_of(e), places = places_of(e);
-    const int tile = (int)((at - b_first) / places), place = (int)((at - b_first) % places);
+    int place;
+    const int tile = (int)divide(at - b_first, places, place);
     const int left = (int)((long long)(places - place) < end - at ? places - place : end - at);  // places of the share in this tile
     const int tiles = row_tiles<C::kRows>(p, e);
     const int head = tile / tiles, row_base = (tile % tiles) * C::kRows;
@@ -128,60 +129,45 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
     const int s_begin = max(0, place - kTileCost), s_end = max(0, place + left - kTileCost);
     const int rows = e.n * p.group;
     const bool complete = s_begin == 0 && s_end == steps;
-    if (!WHOLE && lane == 0) {
-      // who begins a tile knows who ends it
-      int2* rec = nullptr;
-      if (s_begin == 0 && s_end > 0) rec = p.records + (p.by_tile ? (size_t)b * p.tiles + tile : (size_t)worker);
-      if (rec && (p.by_tile || !complete)) {
-        const long long t1 = b_first + (long long)(tile + 1) * places;
-        *rec = complete ? make_int2(-1, 0) : make_int2(worker, share_of(total, used, t1 - 1));
-        if (!p.by_tile) p.tile_of[worker] = make_int4(b, tile, 0, 0);
-      }
-    }
+    if (!WHOLE && lane == 0 && s_begin == 0 && s_end > 0)  // who begins a tile knows who ends it
+      leave_record(p, worker, complete, complete ? 0 : deal.worker_of(b_first + (long long)(tile + 1) * places - 1), e, b, tile, head, row_base);
 
    if (s_end > 0) {
     // this lane's rows: as B operand row g of each n-tile, as accumulator column 2t, 2t + 1
     uint32_t qf[NT][kKk][2];
     int limit[NT][2], limit_min = e.len;
+    auto load_rows = [&]() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = row_base + nt * 8 + g;
-      uint4 x[D / 32];
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = row_base + nt * 8 + g;
+        uint4 x[D / 32];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) x[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int token = r / p.group;
-        const __half* src = p.q + (p.e.q_offsets ? (long long)(e.row0 + token) * p.q_token_stride
-                                                 : (long long)b * p.q_batch_stride + (long long)token * p.q_token_stride) +
-                            (long long)(head * p.group + r % p.group) * p.q_head_stride;
+        for (int i = 0; i < D / 32; ++i) x[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+          const int token = r / p.group;
+          const __half* src = p.q + (p.e.q_offsets ? (long long)(e.row0 + token) * p.q_token_stride
+                                                   : (long long)b * p.q_batch_stride + (long long)token * p.q_token_stride) +
+                              (long long)(head * p.group + r % p.group) * p.q_head_stride;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          x[2 * h] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16));
-          x[2 * h + 1] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16 + 8));
+          for (int h = 0; h < D / 64; ++h) {
+            x[2 * h] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16));
+            x[2 * h + 1] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16 + 8));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          qf[nt][2 * i][0] = x[i].x; qf[nt][2 * i][1] = x[i].y;
+          qf[nt][2 * i + 1][0] = x[i].z; qf[nt][2 * i + 1][1] = x[i].w;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int rc = row_base + nt * 8 + 2 * t + c;
+          limit[nt][c] = rc >= rows ? 0 : p.causal ? min(e.len, max(0, e.len - e.n + rc / p.group + 1)) : e.len;
         }
       }
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        qf[nt][2 * i][0] = x[i].x; qf[nt][2 * i][1] = x[i].y;
-        qf[nt][2 * i + 1][0] = x[i].z; qf[nt][2 * i + 1][1] = x[i].w;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int rc = row_base + nt * 8 + 2 * t + c;
-        limit[nt][c] = rc >= rows ? 0 : p.causal ? min(e.len, max(0, e.len - e.n + rc / p.group + 1)) : e.len;
-      }
-    }
-    if (p.causal) limit_min = min(e.len, max(0, e.len - e.n + row_base / p.group + 1));
-
-    float m_ref[NT][2], l_run[NT][2], v_ref = 0.0f;
-    float o[NT][kKk][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
-      l_run[nt][0] = l_run[nt][1] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kKk; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f; }
-    }
+      if (p.causal) limit_min = min(e.len, max(0, e.len - e.n + row_base / p.group + 1));
+    };
+    if (NT > 2) load_rows();  // while the first steps are under way, where there are registers for both
 
     // this warp's steps: s_first + i * kStride, i < count (an entry without keys has none)
     const int s_first = s_begin + (WHOLE ? warp : 0);
@@ -235,6 +221,17 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
     };
 #pragma unroll 1
     for (int i = 0; i < C::kStages - 1; ++i) copy_step(i);
+
+    if (NT <= 2) load_rows();
+    float m_ref[NT][2], l_run[NT][2], v_ref = 0.0f;
+    float o[NT][kKk][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
+      l_run[nt][0] = l_run[nt][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kKk; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f; }
+    }
 
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
@@ -474,7 +471,7 @@ Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a,
   p.workers = tc ? ctas : ctas * kWarps;
   p.by_tile = tiles * a->batch <= p.workers;
   p.records = p.by_tile ? p.tiles * a->batch : p.workers;
-  p.bytes = p.whole ? 0 : (size_t)p.workers * (sizeof(int2) + sizeof(int4)) + (size_t)2 * p.workers * p.rows * (c->head_dim + 2) * sizeof(float);
+  p.bytes = p.whole ? 0 : (size_t)p.workers * sizeof(Kv8Record) + (size_t)2 * p.workers * p.rows * (c->head_dim + 2) * sizeof(float);
   return p;
 }
 
@@ -566,8 +563,7 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   p.workers = pl.workers;
   p.by_tile = pl.by_tile;
   p.parts = (float*)a->scratch;
-  p.tile_of = (int4*)(p.parts + (size_t)2 * pl.workers * pl.rows * (cache->head_dim + 2));
-  p.records = (int2*)(p.tile_of + pl.workers);
+  p.records = (Kv8Record*)(p.parts + (size_t)2 * pl.workers * pl.rows * (cache->head_dim + 2));
   p.status = dev->status_dev;
   cudaStream_t s = (cudaStream_t)stream;
   if (pl.nt == 0) return launch_kv8_attention_tc(p, pl, cache->head_dim, cache->type, dev, s);

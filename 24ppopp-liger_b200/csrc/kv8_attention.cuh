@@ -9,6 +9,14 @@
 
 namespace liger {
 
+// A tile that is split, as the worker that begins it leaves it to the join.
+struct alignas(16) Kv8Record {
+  int first, last;          // the workers that have its first and its last part; first = -1: nothing to join
+  int row0, row_base, rows; // the entry's first token, the tile's first row in the entry, the rows of the entry
+  int head;
+  int pad[2];
+};
+
 struct Kv8AttnParams {
   Kv8Layer c;
   Kv8Entries e;
@@ -22,8 +30,7 @@ struct Kv8AttnParams {
   // shares
   int workers;       // warps or CTAs that share the work
   int by_tile;       // 1: records are numbered by entry and tile, 0: by the worker that began the tile
-  int2* records;     // a tile that is split: the workers that have its first and its last part (else x = -1)
-  int4* tile_of;     // by worker only: the entry, tile of that record
+  Kv8Record* records;
   float* parts;      // [2 * workers] partial results
   DeviceStatus* status;
 };
@@ -69,23 +76,48 @@ __device__ __forceinline__ Entry load_entry(const Kv8AttnParams& p, int b, bool 
 template <int ROWS>
 __device__ __forceinline__ int row_tiles(const Kv8AttnParams& p, const Entry& e) { return (e.n * p.group + ROWS - 1) / ROWS; }
 
+// a / b and a % b, by 32-bit division where that will do (a 64-bit one takes some 200 cycles)
+__device__ __forceinline__ long long divide(long long a, int b, int& rest) {
+  if ((unsigned long long)a >> 32 == 0) {
+    const unsigned q = (unsigned)a / (unsigned)b;
+    rest = (int)((unsigned)a - q * (unsigned)b);
+    return q;
+  }
+  rest = (int)(a % b);
+  return a / b;
+}
+
+// What a worker that begins a tile (first step of it) leaves for the join; `complete`: it also ends it.
+__device__ __forceinline__ void leave_record(const Kv8AttnParams& p, int worker, bool complete, int last, const Entry& e, int b, int tile, int head,
+                                             int row_base) {
+  if (!p.by_tile && complete) return;
+  int4* at = reinterpret_cast<int4*>(p.records + (p.by_tile ? (size_t)b * p.tiles + tile : (size_t)worker));
+  at[0] = make_int4(complete ? -1 : worker, last, e.row0, row_base);
+  at[1] = make_int4(e.n * p.group, head, 0, 0);
+}
+
 __device__ __forceinline__ int workers_used(long long total, int workers, int least) {
-  const long long want = (total + least - 1) / least;
+  int rest;
+  const long long want = divide(total + least - 1, least, rest);
   return (int)(want < workers ? want : workers);
 }
-__device__ __forceinline__ long long share_begin(long long total, int used, int w) { return total * w / used; }
-__device__ __forceinline__ int share_of(long long total, int used, long long at) {  // the worker whose share has place `at`
-  int w = (int)(at * used / total);
-  while (share_begin(total, used, w + 1) <= at) ++w;
-  while (share_begin(total, used, w) > at) --w;
-  return w;
-}
+// How the line is dealt out: the first `more` workers have `each` + 1 places, the others `each`.
+struct Kv8Deal {
+  long long each;
+  int more, used;
+  __device__ __forceinline__ long long begin(int w) const { return each * w + min(w, more); }
+  __device__ __forceinline__ int worker_of(long long at) const {
+    int rest;
+    const long long wide = (each + 1) * more;
+    if (at < wide) return (int)(each + 1 < 0x7fffffff ? divide(at, (int)(each + 1), rest) : at / (each + 1));
+    return more + (int)(each < 0x7fffffff ? divide(at - wide, (int)each, rest) : (at - wide) / each);
+  }
+};
 
 // Where the shares of a CTA's workers begin: entry and that entry's first place (entry -1: no share).
 template <int SHARES>
 struct Kv8Shares {
-  long long total;
-  int used;
+  Kv8Deal deal;
   int b[SHARES];
   long long first[SHARES];
 };
@@ -106,13 +138,15 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < kW; ++w) total += s_warp[w];
-  const int used = workers_used(total, p.workers, least);
-  if (threadIdx.x == 0) { out.total = total; out.used = used; }
+  Kv8Deal deal;
+  deal.used = workers_used(total, p.workers, least);
+  deal.each = divide(total, max(deal.used, 1), deal.more);
+  if (threadIdx.x == 0) out.deal = deal;
   if (threadIdx.x < SHARES) out.b[threadIdx.x] = -1;
   __syncthreads();
   const int w0 = blockIdx.x * SHARES;
-  if (w0 < used) {
-    const long long last = share_begin(total, used, min(w0 + SHARES, used) - 1);  // where the last of the CTA's shares begins
+  if (w0 < deal.used) {
+    const long long last = deal.begin(min(w0 + SHARES, deal.used) - 1);  // where the last of the CTA's shares begins
     long long before = 0;
     for (int base = 0; base < p.e.batch && before <= last; base += THREADS) {
       const int b = base + threadIdx.x;
@@ -134,8 +168,8 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
       const long long lo = before + incl - v, hi = before + incl;
 #pragma unroll
       for (int w = 0; w < SHARES; ++w) {
-        if (w0 + w >= used) break;
-        const long long at = share_begin(total, used, w0 + w);
+        if (w0 + w >= deal.used) break;
+        const long long at = deal.begin(w0 + w);
         if (at >= lo && at < hi) { out.b[w] = b; out.first[w] = lo; }
       }
       before += all;
@@ -150,27 +184,22 @@ constexpr int kJoinRowThreads = 1024, kJoinThreads = 256;
 // Joins the parts of the tiles that are split over several shares.  SHARED: a CTA has one row of a tile, whose parts its 32 warps
 // take in turn; else a warp has a row and takes all its parts.  Maxima, sums and accumulators of eight parts are fetched at once.
 template <int D, int ROWS, int SHARED>
-__global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_attention_join_kernel(const Kv8AttnParams p) {
+__global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_attention_join_kernel(const Kv8AttnParams p, int records, int live) {
   constexpr int kPart = ROWS * (D + 2);
   constexpr int kW = (SHARED ? kJoinRowThreads : kJoinThreads) / 32, kA = D / 32, kBatch = 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int b = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
-  Entry e;
-  if (p.by_tile) e = load_entry(p, b, false);  // does not hang on the first kernel, which has waited for what does
-  wait_for_stream();
-  if (p.by_tile && tile >= p.c.kv_heads * row_tiles<ROWS>(p, e)) return;
-  const int2 rec = p.records[blockIdx.x];
-  if (rec.x < 0) return;
-  if (!p.by_tile) {
-    const int4 at = p.tile_of[blockIdx.x];
-    b = at.x;
-    tile = at.y;
-    e = load_entry(p, b, false);
+  const int which = SHARED ? blockIdx.x : blockIdx.x * kW + warp;  // record and row
+  const int at = which / live, r = which % live;
+  if (p.by_tile && at < records) {
+    // tiles that the entry does not have left no record (this does not hang on the first kernel, which has waited for what does)
+    const Entry e = load_entry(p, at / p.tiles, false);
+    if (at % p.tiles >= p.c.kv_heads * row_tiles<ROWS>(p, e)) records = 0;
   }
-  const int r = SHARED ? blockIdx.y : blockIdx.y * kW + warp;
-  const int tiles = row_tiles<ROWS>(p, e);
-  const int head = tile / tiles, row = (tile % tiles) * ROWS + r;
-  if (r >= ROWS || row >= e.n * p.group) return;  // the whole CTA where it shares a row
+  wait_for_stream();
+  if (at >= records) return;
+  const int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
+  const int row = rec.w + r, rows = rec2.x, head = rec2.y;
+  if (rec.x < 0 || row >= rows) return;  // the whole CTA where it shares a row
   const int first = rec.x + (SHARED ? warp : 0);
   constexpr int kStride = SHARED ? kW : 1;
   float m = -INFINITY, l = 0.0f, a[kA];
@@ -218,7 +247,7 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
     m = m_new;
   }
   const int token = row / p.group;
-  __half* out = p.out + (size_t)(e.row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
+  __half* out = p.out + (size_t)(rec.z + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
   if (!SHARED) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (D == 128)
@@ -250,11 +279,12 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
 // Few tiles are split into many parts each: a CTA for each of their rows.
 template <int D, int ROWS>
 int launch_join(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
-  if ((long long)pl.records * pl.live <= 2 * dev->sm_count)
-    return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 1>, dim3(pl.records, pl.live), kJoinRowThreads, 0, s, ap);
-  constexpr int kRows = kJoinThreads / 32;
-  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 0>, dim3(pl.records, (pl.live + kRows - 1) / kRows),
-                      kJoinThreads, 0, s, ap);
+  const unsigned rows = (unsigned)pl.records * pl.live;
+  if (rows <= 2u * dev->sm_count)
+    return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 1>, dim3(rows), kJoinRowThreads, 0, s, ap, pl.records, pl.live);
+  constexpr unsigned kRows = kJoinThreads / 32;
+  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 0>, dim3((rows + kRows - 1) / kRows), kJoinThreads, 0, s, ap,
+                      pl.records, pl.live);
 }
 
 #endif

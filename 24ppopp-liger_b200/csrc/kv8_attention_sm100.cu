@@ -219,8 +219,8 @@ struct Walk {
   __device__ __forceinline__ void start(const Kv8AttnParams& p, const Kv8Shares<1>& sh) {
     valid = sh.b[0] >= 0;
     if (!valid) return;
-    at = share_begin(sh.total, sh.used, blockIdx.x);
-    end = share_begin(sh.total, sh.used, blockIdx.x + 1);
+    at = sh.deal.begin(blockIdx.x);
+    end = sh.deal.begin(blockIdx.x + 1);
     b = sh.b[0];
     e = load_entry(p, b, false);
     const long long inside = at - sh.first[0], per = head_places(p, e);
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
       bool ok = true;
       Walk walk;
       walk.start(p, shares);
-      if (!p.by_tile && lane == 0) p.records[worker].x = -1;
+      if (!p.by_tile && lane == 0) p.records[worker].first = -1;
       // hands the walk's tile out and goes on to the next
       auto hand_out = [&]() {
         const uint32_t i = given & 3u;
@@ -520,12 +520,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
             s.head = walk.head; s.rt = walk.rt; s.s0 = walk.s0; s.s1 = walk.s1; s.stop0 = walk.stop(0); s.stop1 = walk.stop(1);
             s.complete = walk.complete();
             s.part = 2 * worker + (walk.first && walk.s0 > 0 ? 0 : 1);
-            if (s.s0 == 0 && s.s1 > 0 && (p.by_tile || !s.complete)) {  // who begins a tile knows who ends it
-              const int tile = s.head * tiles_of(p, walk.e) + s.rt;
-              p.records[p.by_tile ? (size_t)s.b * p.tiles + tile : (size_t)worker] =
-                  s.complete ? make_int2(-1, 0) : make_int2(worker, share_of(shares.total, shares.used, walk.tile0 + walk.t.places() - 1));
-              if (!p.by_tile) p.tile_of[worker] = make_int4(s.b, tile, 0, 0);
-            }
+            if (s.s0 == 0 && s.s1 > 0)  // who begins a tile knows who ends it
+              leave_record(p, worker, s.complete, s.complete ? 0 : shares.deal.worker_of(walk.tile0 + walk.t.places() - 1), walk.e, s.b,
+                           s.head * tiles_of(p, walk.e) + s.rt, s.head, s.rt * kItemRows);
           }
           segments[i] = s;
         }
