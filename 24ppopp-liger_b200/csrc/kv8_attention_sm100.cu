@@ -451,16 +451,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
 #pragma unroll 1
         for (int j = s0 - 1; j < stop && ok; ++j) {
           const uint32_t n = g + (uint32_t)(j - s0);
+          // the tiles first, so that nothing but the weights stands between them and the products
+          if ((j >= s0 && !bar_wait(v_full + (n & 1u) * 8, (n >> 1) & 1u, abort_flag)) ||
+              (j + 1 < stop && !bar_wait(k_full + ((n + 1) & 1u) * 8, ((n + 1) >> 1) & 1u, abort_flag))) { ok = false; break; }
+          fence_proxy_async();  // V, K
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             const int end = h ? e1 : e0;
             if (j >= s0 && j < end) {
               const uint32_t st = n & 1u;
-              if (!bar_wait(v_full + st * 8, (n >> 1) & 1u, abort_flag) || !bar_wait(p_full + h * 8, (np >> h) & 1u, abort_flag) ||
-                  (j == s0 && !bar_wait(o_empty + h * 8, ((no >> h) & 1u) ^ 1u, abort_flag))) { ok = false; break; }
+              if (!bar_wait(p_full + h * 8, (np >> h) & 1u, abort_flag) || (j == s0 && !bar_wait(o_empty + h * 8, ((no >> h) & 1u) ^ 1u, abort_flag))) { ok = false; break; }
               np ^= 1u << h;
               if (j == s0) no ^= 1u << h;
-              fence_proxy_async();  // V
               tc_fence_after();
               if (elect_one()) {
                 const uint32_t va = sV + st * C::kTile, o = tmem + 256 + h * 128, pa = tmem + h * 128;
@@ -473,10 +475,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
             }
             if (j + 1 < end) {
               const uint32_t m = n + 1, st = m & 1u;
-              if (!bar_wait(k_full + st * 8, (m >> 1) & 1u, abort_flag) ||
-                  (j < s0 && !bar_wait(q_full + h * 8, (nq >> h) & 1u, abort_flag))) { ok = false; break; }
-              if (j < s0) nq ^= 1u << h;
-              fence_proxy_async();  // Q, K
+              if (j < s0) {
+                if (!bar_wait(q_full + h * 8, (nq >> h) & 1u, abort_flag)) { ok = false; break; }
+                nq ^= 1u << h;
+                fence_proxy_async();
+              }
               tc_fence_after();
               if (elect_one()) {
                 const uint32_t qa = sQ + h * C::kTile, ka = sK + st * C::kTile;

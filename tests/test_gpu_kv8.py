@@ -41,10 +41,10 @@ def attend_args(liger, cache, q, out, lens, heads, q_len, batch, offsets=None, s
 
 
 def check_attention(got, cache, q, at, lens, slots, scale, causal, layer=0, what="", q_len=None):
-    """`q_len`: the call's bound on new tokens; with more than 24 rows a key head the weights are single fp16 numbers."""
+    """`q_len`: the call's bound on new tokens; with more than 48 rows a key head the weights are single fp16 numbers."""
     heads, d = q.shape[1], q.shape[2]
     q_len = q_len or max(max(b - a for a, b in zip(at, at[1:])), 1)
-    many_rows = q_len * (heads // cache.kv_heads) > 24
+    many_rows = q_len * (heads // cache.kv_heads) > 48
     for b, length in enumerate(lens):
         lo, hi = at[b], at[b + 1]
         want, mixed, size, top = attention(cache, layer, q[lo:hi], hi - lo, length, slots[b], scale, causal)
