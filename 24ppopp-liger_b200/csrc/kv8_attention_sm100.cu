@@ -255,7 +255,6 @@ struct Walk {
   }
   // blocks of half h in this share: [s0, stop(h))
   __device__ __forceinline__ int stop(int h) const { return max(s0, min(s1, h ? t.n1 : t.n0)); }
-  __device__ __forceinline__ int stop() const { return max(stop(0), stop(1)); }
   __device__ __forceinline__ bool complete() const { return s0 == 0 && s1 == max(1, t.blocks()); }
 };
 
@@ -671,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         const int cut = limit - j * kBlock - cp * 64;  // this thread's columns from here on are not seen
         // groups of 16 columns: the first `free` are seen by all rows of the warp (none, where a page is missing or a scale is 0 or not
         // finite), those from `shut` on by none
-        const int free = rf.z == 0.0f ? (limit_low - j * kBlock - cp * 64) >> 4 : 0;
+        const int free = rf.z == 0.0f ? min(4, (limit_low - j * kBlock - cp * 64) >> 4) : 0;
         const int shut = min(4, (limit_high - j * kBlock - cp * 64 + 15) >> 4);
         // the rows' largest scores, in log2 units and without the value scales; the two warps of a row tell each other
         float mx = -INFINITY;
