@@ -42,6 +42,11 @@ __device__ __forceinline__ void wait_for_stream() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+// What may have been written by the predecessor is read with ordinary loads: the read-only path is for data that does not change
+// while the grid lives, and the grid begins before its predecessor ends.
+template <typename T>
+__device__ __forceinline__ T kv8_ld(const T* p) { return *p; }
+
 template <typename... Params, typename... Args>
 int launch_early(const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg{};
@@ -79,7 +84,7 @@ __device__ __forceinline__ bool kv8_rows(const Kv8Entries& e, int b, int& n, int
     row0 = b * e.q_len;
     return true;
   }
-  const int lo = __ldg(e.q_offsets + b), hi = __ldg(e.q_offsets + b + 1);
+  const int lo = kv8_ld(e.q_offsets + b), hi = kv8_ld(e.q_offsets + b + 1);
   if (lo < 0 || hi < lo || hi > e.total_tokens || hi - lo > e.q_len) {
     n = 0;
     row0 = 0;
@@ -90,7 +95,7 @@ __device__ __forceinline__ bool kv8_rows(const Kv8Entries& e, int b, int& n, int
   return true;
 }
 
-__device__ __forceinline__ int kv8_slot(const Kv8Entries& e, int b) { return e.slots ? __ldg(e.slots + b) : b; }
+__device__ __forceinline__ int kv8_slot(const Kv8Entries& e, int b) { return e.slots ? kv8_ld(e.slots + b) : b; }
 
 // ---- codes ----------------------------------------------------------------------------------------------------------------
 // fp32 -> code, round to nearest even; e4m3 saturates, int8 wants what rounds to -127 .. 127

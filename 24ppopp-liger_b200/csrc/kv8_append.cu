@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   int n, row0;
   const bool rows_ok = kv8_rows(p.e, b, n, row0);
   const int slot = kv8_slot(p.e, b);
-  const int pos0 = __ldg(p.positions + b);
+  const int pos0 = kv8_ld(p.positions + b);
   const bool lead = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
   if (!rows_ok || n == 0) {
     if (lead && !rows_ok) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend, b, 0);
@@ -124,9 +124,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
     if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 1, b, (unsigned)slot);
     return;
   }
-  if (p.e.slots) {  // an earlier entry of the same slot has it
+  if (p.e.slots) {  // an earlier entry of the same slot that brings tokens has it
     bool dup = false;
-    for (int j = threadIdx.x; j < b; j += kAppendThreads) dup |= __ldg(p.e.slots + j) == slot;
+    for (int j = threadIdx.x; j < b; j += kAppendThreads)
+      dup |= kv8_ld(p.e.slots + j) == slot && (p.e.q_offsets == nullptr || kv8_ld(p.e.q_offsets + j + 1) > kv8_ld(p.e.q_offsets + j));
     if (__syncthreads_or(dup)) {
       if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 2, b, (unsigned)slot);
       return;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   bool active = wanted;
   int page = -1;
   if (active) {
-    page = __ldg(p.c.table + (size_t)slot * p.c.max_pages + (start >> p.c.page_shift));
+    page = kv8_ld(p.c.table + (size_t)slot * p.c.max_pages + (start >> p.c.page_shift));
     if (page < 0 || page >= p.c.num_pages) {
       if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 3, b, (unsigned)page);
       active = false;

@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
                               (long long)(head * p.group + r % p.group) * p.q_head_stride;
 #pragma unroll
           for (int h = 0; h < D / 64; ++h) {
-            x[2 * h] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16));
-            x[2 * h + 1] = __ldg(reinterpret_cast<const uint4*>(src + h * 64 + t * 16 + 8));
+            x[2 * h] = kv8_ld(reinterpret_cast<const uint4*>(src + h * 64 + t * 16));
+            x[2 * h + 1] = kv8_ld(reinterpret_cast<const uint4*>(src + h * 64 + t * 16 + 8));
           }
         }
 #pragma unroll
@@ -188,15 +188,15 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
       ks = vs = 0.0f;
       if (i < count) {
         const int key = (s_first + i * kStride) * kStep;
-        page = __ldg(row_table + (key >> p.c.page_shift));
+        page = kv8_ld(row_table + (key >> p.c.page_shift));
         if (page < 0 || page >= p.c.num_pages) {
           report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 2, b, (unsigned)page);
           page = -1;
         } else {
           const size_t ph = (size_t)page * p.c.kv_heads + head;
           const size_t blk = (ph << (p.c.page_shift - p.c.block_shift)) + ((key & page_mask) >> p.c.block_shift);
-          ks = __ldg(p.c.ks + blk);
-          vs = __ldg(p.c.vs + blk);
+          ks = kv8_ld(p.c.ks + blk);
+          vs = kv8_ld(p.c.vs + blk);
           if (!(ks >= 0.0f && ks < INFINITY)) ks = NAN;
           if (!(vs >= 0.0f && vs < INFINITY)) vs = NAN;
         }
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
     if (at < end && at == b_first + (long long)p.c.kv_heads * tiles * places) {
       b_first = at;
       do {
-        ++b;
+        if (++b >= p.e.batch) return;  // only if the lengths changed under the call
         e = load_entry(p, b, false);
       } while (e.n == 0);  // entries without new tokens have no place in the line
     }
@@ -572,6 +572,7 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   const DeviceInfo* dev = nullptr;
   if ((rc = require_sm100(&dev)) != LIGER_OK) return rc;
   const Kv8AttnPlan pl = plan_of(cache, a, dev->sm_count);
+  if (pl.bytes && !a->scratch) return set_error(LIGER_ERR_INVALID, "kv8_attention: scratch is NULL");
   if (a->scratch_bytes < pl.bytes)
     return set_error(LIGER_ERR_TOO_LARGE, "kv8_attention: scratch has %zu bytes, %zu are needed", a->scratch_bytes, pl.bytes);
   if (pl.tiles == 0x7fffffff) return set_error(LIGER_ERR_UNSUPPORTED, "kv8_attention: q_len %d x heads %d is too large", a->q_len, a->heads);

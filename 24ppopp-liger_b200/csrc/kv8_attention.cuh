@@ -65,7 +65,7 @@ struct Entry {
 __device__ __forceinline__ Entry load_entry(const Kv8AttnParams& p, int b, bool report) {
   Entry e;
   if (!kv8_rows(p.e, b, e.n, e.row0) && report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention, b, 0);
-  e.len = __ldg(p.kv_lens + b);
+  e.len = kv8_ld(p.kv_lens + b);
   e.slot = kv8_slot(p.e, b);
   if (e.len < 0 || e.len > p.max_kv_len || e.slot < 0 || e.slot >= p.c.slots || e.len > ((long long)p.c.max_pages << p.c.page_shift)) {
     if (report) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAttention + 1, b, (unsigned)e.len);

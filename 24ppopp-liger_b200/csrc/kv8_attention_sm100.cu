@@ -95,7 +95,7 @@ __device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
 // codes are read once: past L1, which is small here and holds what registers cannot
 __device__ __forceinline__ uint4 load_code(const uint8_t* at) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
   return v;
 }
 __device__ __forceinline__ void sts32(uint32_t at, float x) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
@@ -246,7 +246,10 @@ struct Walk {
       if (++head == p.c.kv_heads) {
         head = 0;
         do {
-          ++b;
+          if (++b >= p.e.batch) {  // only if the lengths changed under the call
+            valid = false;
+            return;
+          }
           e = load_entry(p, b, false);
         } while (e.n == 0);
       }
@@ -265,7 +268,7 @@ struct Lookup {
   int head, len, stop, page_mask, lane;
   __device__ __forceinline__ int page(int j) const {
     const int key = j * kBlock + (lane & 7) * 16;
-    return lane < 16 && j < stop && key < len ? __ldg(row_table + (key >> p.c.page_shift)) : -1;
+    return lane < 16 && j < stop && key < len ? kv8_ld(row_table + (key >> p.c.page_shift)) : -1;
   }
   // -1 for a page that does not exist; told once, by the warp that has a status to tell
   __device__ __forceinline__ int valid(int page, int j, DeviceStatus* status, int b) const {
@@ -277,7 +280,7 @@ struct Lookup {
     if (page < 0) return 0.0f;
     const int key = j * kBlock + (lane & 7) * 16;
     const size_t ph = (size_t)page * p.c.kv_heads + head;
-    return __ldg((lane < 8 ? p.c.ks : p.c.vs) + (ph << (p.c.page_shift - p.c.block_shift)) + ((key & page_mask) >> p.c.block_shift));
+    return kv8_ld((lane < 8 ? p.c.ks : p.c.vs) + (ph << (p.c.page_shift - p.c.block_shift)) + ((key & page_mask) >> p.c.block_shift));
   }
 };
 

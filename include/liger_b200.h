@@ -265,7 +265,8 @@ typedef struct liger_kv8_cache {
  * of the sequence keeps its scale unless the new one is larger, and its codes are then rounded again to the larger scale.
  * code = round-to-nearest-even(fp32(x * fp32(1 / scale))), saturated.  A block of zeros has scale 0.
  * The pages have to be there (liger_kv8_reserve) and belong to the slot alone from positions[b] on (liger_kv8_fork sees
- * to that).  A slot that is named twice in one call is written for its first entry only (LIGER_DEV_BAD_INDEX).
+ * to that).  A slot that two entries with tokens name is written for the first of them only
+ * (LIGER_DEV_BAD_INDEX).
  * Strides are multiples of 8 elements, k and v 16-byte aligned.
  */
 typedef struct liger_kv8_append_args {

@@ -732,3 +732,141 @@ def test_a_serving_run(gpu, liger, kind):
     got = cache.from_gpu()
     assert all(torch.equal(got[n], getattr(cache, n)) for n in ("table", "count", "refs"))
     status(gpu)
+
+
+# ---- calls that padding, capturing and several streams make ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("group", [1, 40])
+def test_a_call_in_which_nobody_brings_tokens(gpu, liger, group):
+    """A batch of padding only: no rows, and nothing is written."""
+    cache = Cache("int8", num_pages=20, kv_heads=2, page_size=16, head_dim=64, slots=3, max_pages=200)
+    cache.give_pages([40, 0, 17])
+    cache.fill([40, 0, 17])
+    cache.to_gpu(liger)
+    q = torch.zeros((1, 2 * group, 64), dtype=torch.float16, device="cuda")
+    out = torch.full((1, 128 * group), 7.0, dtype=torch.float16, device="cuda")
+    dl, do = ints([40, 0, 17]), ints([0, 0, 0, 0])
+    for q_len in (1, 5):
+        a = attend_args(liger, cache, q, out, dl, 2 * group, q_len, 3, offsets=do, total=0, max_len=3000)
+        liger.check(gpu.liger_kv8_attention(cache.by, C.byref(a), stream_ptr()))
+    b = liger.Kv8AppendArgs()
+    b.k, b.v, b.q_offsets, b.positions, b.batch, b.q_len = q.data_ptr(), q.data_ptr(), do.data_ptr(), dl.data_ptr(), 3, 4
+    b.token_stride, b.head_stride = 128, 64
+    liger.check(gpu.liger_kv8_append(cache.by, C.byref(b), stream_ptr()))
+    status(gpu)
+    assert bool((out == 7.0).all())
+    same_cache(cache)
+
+
+def test_padding_entries_that_name_a_slot_in_use(gpu, liger):
+    """Entries without tokens may name any slot, also one that a later entry writes to."""
+    cache = Cache("e4m3", num_pages=12, kv_heads=2, page_size=32, scale_block=16, head_dim=64, slots=3, max_pages=4)
+    cache.give_pages([96, 96, 96])
+    cache.fill([20, 30, 40])
+    cache.to_gpu(liger)
+    run_append(gpu, liger, cache, [0, 20, 0, 30, 0], [0, 3, 0, 18, 0], slots=[0, 0, 1, 1, 1])
+    status(gpu)
+
+
+@pytest.mark.parametrize("q_len", [1, 60])
+def test_a_captured_step_with_a_branch(gpu, liger, q_len):
+    """reserve, append and attention captured behind work of another stream, replayed with other values in the same buffers."""
+    h, d, ps = 2, 128, 32
+    cache = Cache("int8", num_pages=40, kv_heads=h, page_size=ps, scale_block=32, head_dim=d, slots=2, max_pages=16)
+    cache.to_gpu(liger)
+    pages = Pages(40, 2, 16, ps)
+    gen = torch.Generator().manual_seed(3)
+    hk, hv, hq = (torch.randn((3, 2 * q_len, h, d), generator=gen).half() for _ in range(3))
+    k, v, q = (x.cuda() for x in (hk, hv, hq))
+    now_k, now_v, now_q = (torch.zeros_like(x[0]) for x in (k, v, q))
+    lens, first, slots, step = ints([0, 0]), ints([0, 0]), ints([0, 1]), torch.zeros(1, dtype=torch.int64, device="cuda")
+    out = torch.zeros((2 * q_len, h * d), dtype=torch.float16, device="cuda")
+    space = torch.empty(gpu.liger_kv8_pages_scratch_bytes(cache.by, 2), dtype=torch.uint8, device="cuda")
+    a = liger.Kv8AppendArgs()
+    a.k, a.v, a.positions, a.batch, a.q_len = now_k.data_ptr(), now_v.data_ptr(), first.data_ptr(), 2, q_len
+    a.batch_stride, a.token_stride, a.head_stride = q_len * h * d, h * d, d
+    b = attend_args(liger, cache, now_q, out, lens, h, q_len, 2, max_len=500)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            now_q.copy_(q.index_select(0, step)[0])
+        now_k.copy_(k.index_select(0, step)[0])
+        now_v.copy_(v.index_select(0, step)[0])
+        first.copy_(lens)
+        lens.add_(q_len)
+        liger.check(gpu.liger_kv8_reserve(cache.by, ptr(slots), ptr(lens), 2, None, ptr(space), space.numel(), stream_ptr()))
+        liger.check(gpu.liger_kv8_append(cache.by, C.byref(a), stream_ptr()))
+        main.wait_stream(side)
+        liger.check(gpu.liger_kv8_attention(cache.by, C.byref(b), stream_ptr()))
+        step.add_(1)
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        length = (i + 1) * q_len
+        pages.reserve([0, 1], [length, length])
+        cache.table, cache.count, cache.refs = pages.arrays()
+        for s in range(2):
+            rows = slice(s * q_len, (s + 1) * q_len)
+            append(cache, 0, s, i * q_len, hk[i, rows], hv[i, rows])
+        same_cache(cache)
+        check_attention(out.cpu(), cache, hq[i], [0, q_len, 2 * q_len], [length] * 2, [0, 1], d ** -0.5, 1, q_len=q_len)
+    status(gpu)
+
+
+def test_long_calls_on_two_streams_at_once(gpu, liger):
+    lens = [2500, 700]
+    cache = Cache("e4m3", num_pages=60, kv_heads=2, page_size=64, scale_block=32, head_dim=64, slots=2, max_pages=45)
+    cache.give_pages(lens)
+    cache.fill(lens)
+    cache.to_gpu(liger)
+    dl = ints(lens)
+    q = [torch.randn((2 * 200, 4, 64), generator=torch.Generator().manual_seed(i)).half() for i in range(2)]
+    dq = [x.cuda() for x in q]
+    out = [torch.zeros((400, 256), dtype=torch.float16, device="cuda") for _ in range(2)]
+    args = [attend_args(liger, cache, dq[i], out[i], dl, 4, 200, 2) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i in range(2):
+            liger.check(gpu.liger_kv8_attention(cache.by, C.byref(args[i]), C.c_void_p(streams[i].cuda_stream)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        check_attention(out[i].cpu(), cache, q[i], [0, 200, 400], lens, [0, 1], 64 ** -0.5, 1)
+    status(gpu)
+
+
+def test_projection_append_and_attention_in_a_row(gpu, liger):
+    """The QKV projection's epilogue writes [B, h, 1, D]; its keys and values go into the cache and its queries look at it, as in a
+    decode step, nothing waiting between."""
+    B, h, d, H = 4, 3, 128, 256
+    lens = [100, 7, 0, 63]
+    cache = Cache("int8", num_pages=16, kv_heads=h, page_size=32, scale_block=16, head_dim=d, slots=B, max_pages=5)
+    cache.give_pages([n + 1 for n in lens])
+    cache.fill(lens)
+    cache.to_gpu(liger)
+    gen = torch.Generator().manual_seed(6)
+    x, w = torch.randn((B, H), generator=gen).half().cuda(), (torch.randn((3 * h * d, H), generator=gen) * 0.06).half().cuda()
+    q, k, v = (torch.zeros((B, h, 1, d), dtype=torch.float16, device="cuda") for _ in range(3))
+    g = liger.GemmArgs()
+    g.a, g.wt, g.q_out, g.k_out, g.v_out = x.data_ptr(), w.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr()
+    g.m, g.n, g.k, g.lda, g.ldw, g.n_end, g.epilogue = B, 3 * h * d, H, H, H, 3 * h * d, liger.capi.EPI_QKV_SPLIT
+    g.seq_len, g.heads, g.head_dim = 1, h, d
+    first, after = ints(lens), ints([n + 1 for n in lens])
+    out = torch.zeros((B, h * d), dtype=torch.float16, device="cuda")
+    a = liger.Kv8AppendArgs()
+    a.k, a.v, a.positions, a.batch, a.q_len = k.data_ptr(), v.data_ptr(), first.data_ptr(), B, 1
+    a.batch_stride, a.token_stride, a.head_stride = h * d, d, d
+    b = attend_args(liger, cache, q, out, after, h, 1, B, strides=(h * d, d, d))
+    liger.check(gpu.liger_gemm_fp16(C.byref(g), stream_ptr()))
+    liger.check(gpu.liger_kv8_append(cache.by, C.byref(a), stream_ptr()))
+    liger.check(gpu.liger_kv8_attention(cache.by, C.byref(b), stream_ptr()))
+    status(gpu)
+    hq, hk, hv = (t.cpu()[:, :, 0] for t in (q, k, v))
+    assert float(hk.abs().max()) > 0.5
+    for s in range(B):
+        append(cache, 0, s, lens[s], hk[s:s + 1], hv[s:s + 1])
+    same_cache(cache)
+    check_attention(out.cpu(), cache, hq, list(range(B + 1)), [n + 1 for n in lens], list(range(B)), d ** -0.5, 1)
