@@ -27,6 +27,7 @@ int kv8_check(const char* what, const liger_kv8_cache* c, int layer) {
     return set_error(LIGER_ERR_UNSUPPORTED, "%s: page_size %d (powers of two from 16 to 256 are implemented)", what, c->page_size);
   if (c->scale_block < 16 || c->scale_block > 128 || c->scale_block > c->page_size || (c->scale_block & (c->scale_block - 1)))
     return set_error(LIGER_ERR_UNSUPPORTED, "%s: scale_block %d (powers of two from 16 to 128, at most page_size)", what, c->scale_block);
+  if (c->num_pages > (1 << 30) || c->slots > (1 << 30)) return set_error(LIGER_ERR_UNSUPPORTED, "%s: num_pages and slots <= 2^30", what);
   if (c->kv_heads > 65535 || (long long)c->max_pages * c->page_size > (1ll << 30))
     return set_error(LIGER_ERR_UNSUPPORTED, "%s: kv_heads <= 65535, max_pages * page_size <= 2^30", what);
   if (layer >= c->layers) return set_error(LIGER_ERR_INVALID, "%s: layer %d of %d", what, layer, c->layers);

@@ -21,6 +21,8 @@
 // goes to scratch and a second, small kernel joins the parts; it is launched early and waits for the first.  Short calls with few
 // tiles give each tile to the eight warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
 // stages of its own with 16-byte asynchronous copies.
+#include <cfloat>
+
 #include "kv8_attention.cuh"
 
 namespace liger {
@@ -34,6 +36,9 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 // Rows a key head up to which this kernel is taken.  A tile has 24 at most, and the cache is read once for each: 48 rows over 12 x
 // 4000 tokens, 8 heads of 128, int8 take 75 us here and 84 us in kv8_attention_tc_kernel, 64 rows 103 and 75.
 constexpr int kFewRows = 48;
+// The warps of kv8_attention_tc_kernel wait for one another over a whole tile at most, and not longer than the wait budget of 2 s: this
+// many keys take 0.3 s.  Calls whose sequences may be longer stay with this kernel, whose warps do not wait.
+constexpr int kLongTile = 1 << 25;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int NT, int WHOLE>
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
         }
         // weights.  The value scale relative to the reference; the reference moves by powers of 16
         float rel = vs * v_back;
-        if (!(rel <= 16.0f && rel >= 0.0625f) && vs > 0.0f) {
+        if (!(rel <= 16.0f && rel >= 0.0625f) && vs > fmaxf(v_ref * kScaleVanishes, FLT_MIN)) {
           const float back = v_ref / vs;  // 0 the first time
           v_ref = vs;
           v_back = 1.0f / vs;
@@ -491,7 +496,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
 Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm_count) {
   Kv8AttnPlan p;
   const long long rows = (long long)a->q_len * (a->heads / c->kv_heads);
-  const bool tc = rows > kFewRows && a->scale > 0.0f;
+  const bool tc = rows > kFewRows && a->scale > 0.0f && a->max_kv_len <= kLongTile;
   p.nt = tc ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
   p.rows = tc ? 256 : 8 * p.nt;
   p.live = (int)(rows < p.rows ? rows : p.rows);

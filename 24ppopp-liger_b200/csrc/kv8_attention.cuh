@@ -179,6 +179,10 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
   __syncthreads();
 }
 
+// A value scale this much below the reference is taken for 0: in a result of fp16 such values do not show beside it, and the ratio's
+// inverse might overflow.
+constexpr float kScaleVanishes = 8.6736174e-19f;  // 2^-60
+
 constexpr int kJoinRowThreads = 1024, kJoinThreads = 256;
 
 // Joins the parts of the tiles that are split over several shares.  SHARED: a CTA has one row of a tile, whose parts its 32 warps

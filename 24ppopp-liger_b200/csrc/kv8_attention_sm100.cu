@@ -564,18 +564,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           float moved = 1.0f;
           if (ref == 0.0f) {
             ref = top;
-          } else if (top > 0.0f && (top > ref * 64.0f || top < ref * 0.015625f)) {
+          } else if (top > ref * 64.0f || (top < ref * 0.015625f && top > ref * kScaleVanishes)) {
             moved = ref / top;
             ref = top;
           }
           const float base = ref > 0.0f ? ref : 1.0f;
+          const bool vanishes = page_now >= 0 && vs <= base * kScaleVanishes;
           if (lane < 8)
             sts128(s_scale + ((g & 3u) * 8 + lane) * 16,
                    make_float4(page_now >= 0 ? mine * p.scale_log2 : 0.0f,
-                               page_now < 0 ? -INFINITY : vs > 0.0f ? __log2f(vs / base) : vs == 0.0f ? 0.0f : NAN,
-                               use ? base / vs : vs == 0.0f && page_now >= 0 ? -1.0f : 1.0f, page_now < 0 ? -INFINITY : 0.0f));
-          // scales that are 0 or not finite, pages that are missing: such a block is weighed with care
-          const bool odd = __any_sync(0xffffffffu, lane < 16 && !(mine > 0.0f));
+                               page_now < 0 ? -INFINITY : vanishes ? 0.0f : vs > 0.0f ? __log2f(vs / base) : NAN,
+                               vanishes ? -1.0f : use ? base / vs : 1.0f, page_now < 0 ? -INFINITY : 0.0f));
+          // scales that vanish or are not finite, pages that are missing: such a block is weighed with care
+          const bool odd = __any_sync(0xffffffffu, lane < 16 && (!(mine > 0.0f) || (lane < 8 && vanishes)));
           if (lane == 0) sts128(s_ref + (g & 3u) * 16, make_float4(base, moved, odd ? 1.0f : 0.0f, 0.0f));
           __syncwarp();
           if (lane == 0) {

@@ -1,6 +1,6 @@
 // Keeping the pages of the paged 8-bit cache: reserve, fork, free, copy, compact.
 //
-// Every operator but free is two launches.  A planning kernel of one CTA decides everything that depends on order (who gets
+// Every operator but free and a small reserve is two launches.  A planning kernel of one CTA decides everything that depends on order (who gets
 // which page), with prefix sums over the entries and over the pages' reference counts, and leaves a list of page moves in the
 // workspace.  A second kernel over the whole GPU then carries it out: the entries' table rows and the bytes of the moved
 // pages, which are what costs time (two launches, no trip to the host).  Which page goes where never hangs on timing:
@@ -13,6 +13,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMoveThreads = 256;
 constexpr int kMovePiece = kMoveThreads * 8 * 16;
+constexpr int kMostEntries = 1 << 28;  // of a call: entries times 8 warps stay within 32 bits
 constexpr int kNobody = 0x7fffffff;
 constexpr int kOwnersShared = 8192;   // slots or pages up to which the owners of a call's numbers are kept in shared memory
 constexpr int kFreeShared = 2048;     // free pages handed out that are kept there
@@ -412,12 +413,18 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_compact_kernel(const PagesPa
   move_pages(p);
 }
 
+int check_n(const char* what, int n) {
+  if (n < 0) return set_error(LIGER_ERR_INVALID, "%s: n must not be negative", what);
+  if (n > kMostEntries) return set_error(LIGER_ERR_UNSUPPORTED, "%s: n <= %d", what, kMostEntries);
+  return LIGER_OK;
+}
+
 int pages_params(const char* what, const liger_kv8_cache* c, int n, bool state, void* scratch, size_t scratch_bytes, PagesParams* p,
                  const DeviceInfo** dev) {
   int rc = kv8_check(what, c, -1);
   if (rc != LIGER_OK) return rc;
   if (state && (!c->page_count || !c->page_refs)) return set_error(LIGER_ERR_INVALID, "%s: page_count and page_refs are needed", what);
-  if (n < 0) return set_error(LIGER_ERR_INVALID, "%s: n must not be negative", what);
+  if ((rc = check_n(what, n)) != LIGER_OK) return rc;
   const Workspace w = workspace_of(c, n);
   if (!scratch || ((uintptr_t)scratch & 15u)) return set_error(LIGER_ERR_INVALID, "%s: scratch must be a 16-byte aligned pointer", what);
   if (scratch_bytes < w.bytes)
@@ -474,7 +481,7 @@ unsigned move_grid(const DeviceInfo* dev, const PagesParams& p, long long moves)
 using namespace liger;
 
 extern "C" size_t liger_kv8_pages_scratch_bytes(const liger_kv8_cache* cache, int n) {
-  if (!cache || cache->num_pages <= 0 || cache->slots <= 0 || n < 0) return 0;
+  if (!cache || cache->num_pages <= 0 || cache->slots <= 0 || n < 0 || n > kMostEntries) return 0;
   return workspace_of(cache, n).bytes;
 }
 
@@ -517,8 +524,7 @@ extern "C" int liger_kv8_free(const liger_kv8_cache* cache, const int* slots, in
   int rc = kv8_check("kv8_free", cache, -1);
   if (rc != LIGER_OK) return rc;
   if (!cache->page_count || !cache->page_refs) return set_error(LIGER_ERR_INVALID, "kv8_free: page_count and page_refs are needed");
-  if (n < 0) return set_error(LIGER_ERR_INVALID, "kv8_free: n must not be negative");
-  if (n == 0) return LIGER_OK;
+  if ((rc = check_n("kv8_free", n)) != LIGER_OK || n == 0) return rc;
   if (!slots) return set_error(LIGER_ERR_INVALID, "kv8_free: slots is NULL");
   if ((rc = check_ints("kv8_free", slots, nullptr, nullptr)) != LIGER_OK) return rc;
   const DeviceInfo* dev = current_device();

@@ -198,6 +198,34 @@ def test_zero_scales_large_scores_and_equal_keys(gpu, liger, many):
     status(gpu)
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("many", [1, 140])
+@pytest.mark.parametrize("scales", [(1.0, 1e-40, 1e-30, 1.0, 3e-5, 1e-39), (1e-40, 0.0, 1e-41, 1e-30, 2e-7, 0.5), (0.0, 1e-40, 1e-45, 0.0, 1e-40, 1e-44),
+                                    (40.0, 1e-12, 1e-20, 1e-25, 0.0, 1e-44)])
+def test_value_scales_of_any_size_side_by_side(gpu, liger, kind, many, scales):
+    """Finite scales that append does not write, numbers below the normal ones among them: a block whose values vanish beside another
+    one's adds nothing, and its weights still count."""
+    lens = [90, 37, 320, 16]
+    cache = Cache(kind, num_pages=20, kv_heads=2, page_size=32, scale_block=16, head_dim=64, slots=4, max_pages=16)
+    cache.give_pages(lens)
+    cache.fill(lens)
+    for slot, n in enumerate(lens):
+        for j in range(-(-n // 16)):
+            cache.vs[0, int(cache.table[slot, j // 2]), :, j % 2] = scales[(j + slot) % len(scales)]
+    run_attention(gpu, liger, cache, lens, [many] * 4, heads=4, ragged=False, max_len=5000)
+    status(gpu)
+
+
+def test_a_bound_on_the_lengths_far_above_them(gpu, liger):
+    """Rows for the tensor-core kernel, in a cache that may grow to 2^29 tokens a sequence."""
+    lens, many = [200, 0, 33], [60, 2, 40]
+    cache = Cache("int8", num_pages=20, kv_heads=2, page_size=64, scale_block=16, head_dim=64, slots=3, max_pages=1 << 23)
+    cache.give_pages(lens)
+    cache.fill(lens)
+    run_attention(gpu, liger, cache, lens, many, heads=4, max_len=1 << 29)
+    status(gpu)
+
+
 @pytest.mark.parametrize("many", [1, 140])
 def test_values_that_are_not_finite_reach_only_those_who_see_them(gpu, liger, many):
     """A NaN block's rows are NaN; rows before it in causal order, other heads and other sequences are not."""

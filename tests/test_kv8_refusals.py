@@ -44,7 +44,8 @@ BAD_CACHES = [(dict(k_pages=None), INVALID, "NULL"), (dict(v_scales=None), INVAL
               (dict(page_size=8), UNSUPPORTED, "page_size"), (dict(page_size=512), UNSUPPORTED, "page_size"),
               (dict(scale_block=64), UNSUPPORTED, "scale_block"), (dict(scale_block=8), UNSUPPORTED, "scale_block"),
               (dict(page_size=256, scale_block=256), UNSUPPORTED, "scale_block"), (dict(kv_heads=70000), UNSUPPORTED, "kv_heads"),
-              (dict(max_pages=1 << 27), UNSUPPORTED, "max_pages")]
+              (dict(max_pages=1 << 27), UNSUPPORTED, "max_pages"), (dict(num_pages=(1 << 30) + 1), UNSUPPORTED, "num_pages"),
+              (dict(slots=(1 << 30) + 1), UNSUPPORTED, "slots")]
 
 
 @pytest.mark.parametrize("kw,code,word", BAD_CACHES)
@@ -118,6 +119,12 @@ def test_page_operators_refuse_bad_arguments(liger):
     assert lib.liger_kv8_free(by, OK, 0, None) == 0
     assert lib.liger_kv8_free(by, None, 2, None) == INVALID
     assert lib.liger_kv8_free(by, OK + 2, 2, None) == INVALID
+    many = (1 << 28) + 1
+    assert lib.liger_kv8_reserve(by, OK, OK, many, OK, OK, 1 << 40, None) == UNSUPPORTED
+    assert lib.liger_kv8_fork(by, OK, OK, OK, many, OK, OK, 1 << 40, None) == UNSUPPORTED
+    assert lib.liger_kv8_copy(by, OK, OK, many, OK, OK, 1 << 40, None) == UNSUPPORTED
+    assert lib.liger_kv8_free(by, OK, many, None) == UNSUPPORTED
+    assert lib.liger_kv8_pages_scratch_bytes(by, many) == 0
     for gone in ("page_count", "page_refs"):
         without = cache(liger, **{gone: None})
         assert lib.liger_kv8_free(C.byref(without), OK, 1, None) == INVALID
