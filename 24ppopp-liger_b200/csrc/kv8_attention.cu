@@ -9,18 +9,28 @@
 //   O^T[dim, row] += V^T P^T A = 16 dims x 16 keys: a lane holds 16 contiguous dims of four keys and pairs the keys' bytes.
 //                            P^T comes out of the S^T accumulators by an 8x8 transpose (movmatrix).
 //
-// Rows are (new token, head of the group) pairs, 8 * NT of them a tile.  Scales: S is multiplied by its key block's scale in
+// Rows are (new token, head of the group) pairs, 4, 8, 16 or 24 of them a tile.  Scales: S is multiplied by its key block's scale in
 // fp32.  The value scale goes into P: w = p * (scale / reference), where the reference follows the scales in powers of
 // 16 (the accumulators are rescaled when it moves), so that w stays where fp16 is precise.  P is split into a leading and a
-// trailing fp16 part, two products, so that its rounding does not show in the result; there is tensor throughput to spare here.  The running
+// trailing fp16 part, two products, so that its rounding does not show in the result.  With at most 4 rows both parts go into one product: columns 4 .. 7
+// are the rows again, with the trailing parts.  (The GPU runs into its power limit here, 1000 W, and the products are what can be saved:
+// 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The running
 // maximum is moved only when some score exceeds it by 2^8, which a warp finds with one vote.
 //
 // Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
-// are; warps never wait for one another.  Where a share begins or ends inside a tile the partial (maximum, sum, accumulator)
-// goes to scratch and a second, small kernel joins the parts; it is launched early and waits for the first.  Short calls with few
+// are; warps do not wait for one another before the end.  Where a share begins or ends inside a tile the partial (maximum, sum,
+// accumulator) goes to scratch and a second, small kernel joins the parts; parts of one tile that neighbouring warps of a CTA have are
+// joined in shared memory first (48 x up to 16384 tokens of 8 heads: 71 -> 65 us).  Short calls with few
 // tiles give each tile to the eight warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
 // stages of its own with 16-byte asynchronous copies.
+//
+// Measured (device time in a row of calls): 32 x 2049 tokens, 96 heads of 128, e4m3: 251 us, 6.4 TB/s (98 % of the copy rate; 271 us over
+// seconds); 48 x up to 16384 tokens, 8 heads of 128 for 64 queries, int8: 65 .. 71 us, 4.5 .. 4.9 TB/s; 2 x 150001 tokens, 4 heads of 128
+// for 20 queries, e4m3: 59 us, 5.2 TB/s.  What the shorter calls miss is some 7 us until the first codes arrive (lengths, table,
+// codes: one after the other) and some 5 us for the join.  5 drafted tokens of 12 sequences behind up to 6000, 8 heads for 32 queries, int8:
+// 42 us, 2.1 TB/s; here the work between the copies is what takes time (29 us without it): 72 products a step of 16 keys, with two warps
+// on a scheduler since 24 rows fill the registers.
 #include <cfloat>
 
 #include "kv8_attention.cuh"
@@ -41,18 +51,19 @@ constexpr int kFewRows = 48;
 constexpr int kLongTile = 1 << 25;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, int NT, int WHOLE>
+// ROWS: of a tile, 4, 8, 16 or 24
+template <int D, int ROWS, int WHOLE>
 struct Cfg {
+  static constexpr int NT = (ROWS + 7) / 8;                          // groups of 8 columns of a product
   static constexpr int kWarps = WHOLE ? kWholeWarps : liger::kWarps;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kRows = 8 * NT;
   static constexpr int kCtas = WHOLE ? 1 : NT == 1 ? 3 : 2;          // resident per SM
   static constexpr int kStage = 2 * kStep * D;                       // K and V of a step
   static constexpr int kStages = (NT == 1 || WHOLE ? 4 : 6) * (128 / D);
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kMerge = kWarps * kRows * (D + 4) * 4;        // accumulators of a CTA's warps, in the place of the rings
+  static constexpr int kMerge = kWarps * ROWS * (D + 4) * 4;         // accumulators of a CTA's warps, in the place of the rings
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kPart = kRows * (D + 2);                      // floats of a partial result: maxima, sums, accumulators
+  static constexpr int kPart = ROWS * (D + 2);                       // floats of a partial result: maxima, sums, accumulators
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -91,9 +102,12 @@ __device__ __forceinline__ int stage_at(int r, int c) {
   return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (r & 6)) << 4);  // two keys a line
 }
 
-template <int D, int TYPE, int NT, int WHOLE>
-__global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>::kCtas) kv8_attention_kernel(const Kv8AttnParams p) {
-  using C = Cfg<D, NT, WHOLE>;
+template <int D, int TYPE, int ROWS, int WHOLE>
+__global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WHOLE>::kCtas) kv8_attention_kernel(const Kv8AttnParams p) {
+  using C = Cfg<D, ROWS, WHOLE>;
+  constexpr int NT = C::NT;
+  constexpr bool kPacked = ROWS == 4;             // columns 4 .. 7 are rows 0 .. 3 again, with the trailing parts of the weights
+  constexpr int kCols = kPacked ? 4 : 8;          // rows of a group of columns
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kKk = D / 16;                     // k-steps of a score product = dim tiles of an output product
   constexpr int kStride = WHOLE ? kWarps : 1;     // the warps of a whole tile take every eighth step
@@ -110,23 +124,28 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
   Kv8Deal deal{};
   const int worker = blockIdx.x * kWarps + warp;
   Entry e;
-  if (WHOLE) {
+  bool grouped = false;
+  __shared__ int s_follows[kWarps], s_rows[kWarps];
+  __shared__ float* s_part[kWarps];
+  if constexpr (WHOLE) {
     b = blockIdx.y;
     e = load_entry(p, b, blockIdx.x == 0 && threadIdx.x == 0);
-    if ((int)blockIdx.x >= p.c.kv_heads * row_tiles<C::kRows>(p, e)) return;
+    if ((int)blockIdx.x >= p.c.kv_heads * row_tiles<ROWS>(p, e)) return;
     at = (long long)blockIdx.x * places_of(e);
     end = at + places_of(e);
   } else {
     __shared__ Kv8Shares<kWarps> shares;
-    find_shares<kThreads>(p, kMinPlaces, [&](const Entry& x) { return line_of<C::kRows>(p, x); }, shares);
+    if (lane == 0) s_follows[warp] = s_rows[warp] = 0;
+    find_shares<kThreads>(p, kMinPlaces, [&](const Entry& x) { return line_of<ROWS>(p, x); }, shares);
     deal = shares.deal;
     b = shares.b[warp];
     b_first = shares.first[warp];
     if (!p.by_tile && lane == 0) p.records[worker].first = -1;
-    if (b < 0) return;
-    at = deal.begin(worker);
-    end = deal.begin(worker + 1);
-    e = load_entry(p, b, false);
+    if (b >= 0) {
+      at = deal.begin(worker);
+      end = deal.begin(worker + 1);
+      e = load_entry(p, b, false);
+    }
   }
   const long long share0 = at;
 
@@ -135,23 +154,26 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
     int place;
     const int tile = (int)divide(at - b_first, places, place);
     const int left = (int)((long long)(places - place) < end - at ? places - place : end - at);  // places of the share in this tile
-    const int tiles = row_tiles<C::kRows>(p, e);
-    const int head = tile / tiles, row_base = (tile % tiles) * C::kRows;
+    const int tiles = row_tiles<ROWS>(p, e);
+    const int head = min(tile / tiles, p.c.kv_heads - 1), row_base = (tile % tiles) * ROWS;
     // a share that ends before a tile's first step leaves the tile to the next
     const int s_begin = max(0, place - kTileCost), s_end = max(0, place + left - kTileCost);
     const int rows = e.n * p.group;
     const bool complete = s_begin == 0 && s_end == steps;
-    if (!WHOLE && lane == 0 && s_begin == 0 && s_end > 0)  // who begins a tile knows who ends it
-      leave_record(p, worker, complete, complete ? 0 : deal.worker_of(b_first + (long long)(tile + 1) * places - 1), e, b, tile, head, row_base);
-
+    // Parts of one tile that neighbouring warps have are joined here: a warp whose share is a tile's inside follows the warp before
+    const long long tile_end = b_first + (long long)(tile + 1) * places;
+    const bool follows = !WHOLE && warp > 0 && at == share0 && s_begin > 0 && end < tile_end;
+    const bool leads = !WHOLE && s_end > 0 && warp + 1 < kWarps && worker + 1 < deal.used && deal.begin(worker + 2) < tile_end;
    if (s_end > 0) {
+    if (!WHOLE && lane == 0 && s_begin == 0)  // who begins a tile knows who ends it
+      leave_record(p, worker, complete, complete ? 0 : deal.worker_of(tile_end - 1), e, b, tile, head, row_base);
     // this lane's rows: as B operand row g of each n-tile, as accumulator column 2t, 2t + 1
     uint32_t qf[NT][kKk][2];
     int limit[NT][2], limit_min = e.len;
     auto load_rows = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = row_base + nt * 8 + g;
+        const int r = row_base + nt * 8 + g % kCols;
         uint4 x[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) x[i] = make_uint4(0, 0, 0, 0);
@@ -173,7 +195,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int rc = row_base + nt * 8 + 2 * t + c;
+          const int rc = row_base + nt * 8 + (2 * t + c) % kCols;
           limit[nt][c] = rc >= rows ? 0 : p.causal ? min(e.len, max(0, e.len - e.n + rc / p.group + 1)) : e.len;
         }
       }
@@ -369,8 +391,9 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
           for (int i = 0; i < 2; ++i) {
             const __half2 hi = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
             const float2 back = __half22float2(hi);
-            ph[nt][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-            pl[nt][i] = transpose8x8(pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y));
+            const uint32_t lead = *reinterpret_cast<const uint32_t*>(&hi), trail = pack_half2(w[2 * i] - back.x, w[2 * i + 1] - back.y);
+            ph[nt][i] = transpose8x8(kPacked && t >= 2 ? trail : lead);
+            if (!kPacked) pl[nt][i] = transpose8x8(trail);
           }
         }
         // O^T += V^T P^T
@@ -397,7 +420,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-              mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+              if (!kPacked) mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
             }
           }
         }
@@ -415,9 +438,16 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
         l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 4);
         l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 8);
         l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 16);
+        if (kPacked) {  // both parts of the weights
+#pragma unroll
+          for (int d = 0; d < kKk; ++d) {
+            o[nt][d][c] += __shfl_xor_sync(0xffffffffu, o[nt][d][c], 2);
+            o[nt][d][c + 2] += __shfl_xor_sync(0xffffffffu, o[nt][d][c + 2], 2);
+          }
+        }
       }
     if (WHOLE) {
-      __shared__ float s_m[kWarps][C::kRows], s_l[kWarps][C::kRows];
+      __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
       float* merge = reinterpret_cast<float*>(smem_kv8);
       __syncthreads();  // the rings are done with
 #pragma unroll
@@ -425,14 +455,15 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int r = nt * 8 + 2 * t + c;
+          if (kPacked && t >= 2) continue;
           if (g == 0) { s_m[warp][r] = m_ref[nt][c]; s_l[warp][r] = l_run[nt][c]; }
-          float* dst = merge + (warp * C::kRows + r) * (D + 4) + g * (D / 8);
+          float* dst = merge + (warp * ROWS + r) * (D + 4) + g * (D / 8);
 #pragma unroll
           for (int d = 0; d < kKk; d += 2)
             *reinterpret_cast<float4*>(dst + 2 * d) = make_float4(o[nt][d][c] * v_ref, o[nt][d][c + 2] * v_ref, o[nt][d + 1][c] * v_ref, o[nt][d + 1][c + 2] * v_ref);
         }
       __syncthreads();
-      for (int i = threadIdx.x; i < C::kRows * D / 4; i += kThreads) {
+      for (int i = threadIdx.x; i < ROWS * D / 4; i += kThreads) {
         const int r = i / (D / 4), d = (i % (D / 4)) * 4;
         if (row_base + r >= rows) break;
         float m = s_m[0][r];
@@ -444,7 +475,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
         for (int w = 0; w < kWarps; ++w) {
           const float lw = s_l[w][r];
           const float f = lw == 0.0f ? 0.0f : lw == lw ? exp2_approx(s_m[w][r] - m) : 1.0f;  // saw nothing / a NaN stays
-          const float4 x = *reinterpret_cast<const float4*>(merge + (w * C::kRows + r) * (D + 4) + d);
+          const float4 x = *reinterpret_cast<const float4*>(merge + (w * ROWS + r) * (D + 4) + d);
           l += f * lw;
           a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
         }
@@ -456,12 +487,22 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
       return;
     }
     float* part = p.parts + (size_t)(2 * worker + (at == share0 && s_begin > 0 ? 0 : 1)) * C::kPart;
+    grouped = follows || leads;
+    if (grouped) {  // in the place of this warp's ring
+      if (lane == 0) {
+        s_follows[warp] = follows;
+        s_rows[warp] = min(ROWS, rows - row_base);
+        s_part[warp] = part;
+      }
+      part = reinterpret_cast<float*>(ring);
+      __syncwarp();
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int r = nt * 8 + 2 * t + c;
-        if (row_base + r >= rows) continue;
+        if (r >= ROWS || row_base + r >= rows) continue;
         if (complete) {
           const int token = (row_base + r) / p.group;
           const float inv = l_run[nt][c] == 0.0f ? 0.0f : v_ref / l_run[nt][c];
@@ -473,8 +514,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
                                                                 pack_half2(o[nt][d + 2][c] * inv, o[nt][d + 2][c + 2] * inv),
                                                                 pack_half2(o[nt][d + 3][c] * inv, o[nt][d + 3][c + 2] * inv));
         } else {
-          if (g == 0) { part[r] = m_ref[nt][c]; part[C::kRows + r] = l_run[nt][c]; }
-          float* dst = part + 2 * C::kRows + r * D + g * (D / 8);
+          if (g == 0) { part[r] = m_ref[nt][c]; part[ROWS + r] = l_run[nt][c]; }
+          float* dst = part + 2 * ROWS + r * D + g * (D / 8);
 #pragma unroll
           for (int d = 0; d < kKk; d += 2)
             *reinterpret_cast<float4*>(dst + 2 * d) = make_float4(o[nt][d][c] * v_ref, o[nt][d][c + 2] * v_ref, o[nt][d + 1][c] * v_ref, o[nt][d + 1][c + 2] * v_ref);
@@ -486,10 +527,41 @@ __global__ void __launch_bounds__(Cfg<D, NT, WHOLE>::kThreads, Cfg<D, NT, WHOLE>
     if (at < end && at == b_first + (long long)p.c.kv_heads * tiles * places) {
       b_first = at;
       do {
-        if (++b >= p.e.batch) return;  // only if the lengths changed under the call
+        if (++b >= p.e.batch) {  // only if the lengths changed under the call
+          e.n = 0;
+          end = at;
+          break;
+        }
         e = load_entry(p, b, false);
       } while (e.n == 0);  // entries without new tokens have no place in the line
     }
+  }
+  if (WHOLE) return;
+
+  // the parts of tiles that neighbouring warps share
+  __syncthreads();
+  if (!grouped) return;
+  int lead = warp, last = warp;
+  while (s_follows[lead]) --lead;
+  while (last + 1 < kWarps && s_follows[last + 1]) ++last;
+  const float* parts = reinterpret_cast<const float*>(smem_kv8);
+  constexpr int kRingFloats = C::kStages * C::kStage / 4;
+  float* part = s_part[lead];
+  for (int i = (warp - lead) * 32 + lane; i < s_rows[lead] * (D / 4); i += (last - lead + 1) * 32) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.0f;
+    for (int w = lead; w <= last; ++w) m = fmaxf(m, parts[w * kRingFloats + r]);
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int w = lead; w <= last; ++w) {
+      const float* q = parts + w * kRingFloats;
+      const float lw = q[ROWS + r];
+      const float f = lw == 0.0f ? 0.0f : lw == lw ? exp2_approx(q[r] - m) : 1.0f;  // saw nothing / a NaN stays
+      const float4 x = *reinterpret_cast<const float4*>(q + 2 * ROWS + r * D + d);
+      l = fmaf(f, lw, l);
+      a.x = fmaf(f, x.x, a.x); a.y = fmaf(f, x.y, a.y); a.z = fmaf(f, x.z, a.z); a.w = fmaf(f, x.w, a.w);
+    }
+    if (d == 0) { part[r] = m; part[ROWS + r] = l; }
+    *reinterpret_cast<float4*>(part + 2 * ROWS + r * D + d) = a;
   }
 }
 
@@ -497,12 +569,11 @@ Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a,
   Kv8AttnPlan p;
   const long long rows = (long long)a->q_len * (a->heads / c->kv_heads);
   const bool tc = rows > kFewRows && a->scale > 0.0f && a->max_kv_len <= kLongTile;
-  p.nt = tc ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
-  p.rows = tc ? 256 : 8 * p.nt;
+  p.rows = tc ? kTcRows : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 24;
   p.live = (int)(rows < p.rows ? rows : p.rows);
   const long long tiles = (long long)c->kv_heads * ((rows + p.rows - 1) / p.rows);
   p.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
-  const int ctas = (tc ? 1 : p.nt == 1 ? 3 : 2) * sm_count;
+  const int ctas = (tc ? 1 : p.rows <= 8 ? 3 : 2) * sm_count;
   p.whole = !tc && a->max_kv_len <= 1024 && tiles * a->batch <= sm_count;
   p.workers = tc ? ctas : ctas * kWarps;
   p.by_tile = tiles * a->batch <= p.workers;
@@ -511,21 +582,25 @@ Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a,
   return p;
 }
 
-template <int D, int TYPE, int NT, int WHOLE>
+template <int D, int TYPE, int ROWS, int WHOLE>
 int launch(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
-  using C = Cfg<D, NT, WHOLE>;
+  using C = Cfg<D, ROWS, WHOLE>;
   static std::atomic<unsigned long long> allowed{0};
-  int rc = allow_smem(kv8_attention_kernel<D, TYPE, NT, WHOLE>, C::kSmem, dev, allowed);
+  int rc = allow_smem(kv8_attention_kernel<D, TYPE, ROWS, WHOLE>, C::kSmem, dev, allowed);
   if (rc != LIGER_OK) return rc;
   const dim3 grid = WHOLE ? dim3(pl.tiles, ap.e.batch) : dim3(pl.workers / kWarps);
-  rc = launch_early("kv8_attention_kernel", kv8_attention_kernel<D, TYPE, NT, WHOLE>, grid, C::kThreads, C::kSmem, s, ap);
-  return rc != LIGER_OK || WHOLE ? rc : launch_join<D, 8 * NT>(ap, pl, dev, s);
+  rc = launch_early("kv8_attention_kernel", kv8_attention_kernel<D, TYPE, ROWS, WHOLE>, grid, C::kThreads, C::kSmem, s, ap);
+  return rc != LIGER_OK || WHOLE ? rc : launch_join<D, ROWS, kWarps>(ap, pl, dev, s);
 }
 
 template <int D, int TYPE>
 int launch_rows(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
-  if (pl.whole) return pl.nt == 1 ? launch<D, TYPE, 1, 1>(ap, pl, dev, s) : pl.nt == 2 ? launch<D, TYPE, 2, 1>(ap, pl, dev, s) : launch<D, TYPE, 3, 1>(ap, pl, dev, s);
-  return pl.nt == 1 ? launch<D, TYPE, 1, 0>(ap, pl, dev, s) : pl.nt == 2 ? launch<D, TYPE, 2, 0>(ap, pl, dev, s) : launch<D, TYPE, 3, 0>(ap, pl, dev, s);
+  switch (pl.rows) {
+    case 4: return pl.whole ? launch<D, TYPE, 4, 1>(ap, pl, dev, s) : launch<D, TYPE, 4, 0>(ap, pl, dev, s);
+    case 8: return pl.whole ? launch<D, TYPE, 8, 1>(ap, pl, dev, s) : launch<D, TYPE, 8, 0>(ap, pl, dev, s);
+    case 16: return pl.whole ? launch<D, TYPE, 16, 1>(ap, pl, dev, s) : launch<D, TYPE, 16, 0>(ap, pl, dev, s);
+    default: return pl.whole ? launch<D, TYPE, 24, 1>(ap, pl, dev, s) : launch<D, TYPE, 24, 0>(ap, pl, dev, s);
+  }
 }
 
 int check_args(const liger_kv8_cache* c, const liger_kv8_attention_args* a) {
@@ -603,7 +678,7 @@ extern "C" int liger_kv8_attention(const liger_kv8_cache* cache, const liger_kv8
   p.records = (Kv8Record*)(p.parts + (size_t)2 * pl.workers * pl.rows * (cache->head_dim + 2));
   p.status = dev->status_dev;
   cudaStream_t s = (cudaStream_t)stream;
-  if (pl.nt == 0) return launch_kv8_attention_tc(p, pl, cache->head_dim, cache->type, dev, s);
+  if (pl.rows == kTcRows) return launch_kv8_attention_tc(p, pl, cache->head_dim, cache->type, dev, s);
   if (cache->head_dim == 128)
     return cache->type == LIGER_KV8_INT8 ? launch_rows<128, LIGER_KV8_INT8>(p, pl, dev, s) : launch_rows<128, LIGER_KV8_E4M3>(p, pl, dev, s);
   return cache->type == LIGER_KV8_INT8 ? launch_rows<64, LIGER_KV8_INT8>(p, pl, dev, s) : launch_rows<64, LIGER_KV8_E4M3>(p, pl, dev, s);

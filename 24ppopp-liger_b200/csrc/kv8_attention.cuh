@@ -36,11 +36,11 @@ struct Kv8AttnParams {
 };
 
 
+constexpr int kTcRows = 256;
 // What a launch takes, as a function of a call's sizes and the SM count alone.
 struct Kv8AttnPlan {
-  int rows;      // rows of a tile
+  int rows;      // rows of a tile; kTcRows: kv8_attention_tc_kernel
   int live;      // rows of a tile that can be in use
-  int nt;        // kv8_attention_kernel's row groups; 0: kv8_attention_tc_kernel
   int tiles;     // most tiles of an entry
   int whole;     // kv8_attention_kernel: a CTA takes a whole tile
   int workers, by_tile, records;
@@ -110,7 +110,8 @@ struct Kv8Deal {
     int rest;
     const long long wide = (each + 1) * more;
     if (at < wide) return (int)(each + 1 < 0x7fffffff ? divide(at, (int)(each + 1), rest) : at / (each + 1));
-    return more + (int)(each < 0x7fffffff ? divide(at - wide, (int)each, rest) : (at - wide) / each);
+    const int w = more + (int)(each < 0x7fffffff ? divide(at - wide, (int)each, rest) : (at - wide) / each);
+    return min(w, used - 1);  // always, unless the lengths change under the call
   }
 };
 
@@ -183,11 +184,13 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
 // inverse might overflow.
 constexpr float kScaleVanishes = 8.6736174e-19f;  // 2^-60
 
-constexpr int kJoinRowThreads = 1024, kJoinThreads = 256;
+constexpr int kJoinRowThreads = 256, kJoinThreads = 256;
 
-// Joins the parts of the tiles that are split over several shares.  SHARED: a CTA has one row of a tile, whose parts its 32 warps
+// Joins the parts of the tiles that are split over several shares.  SHARED: a CTA has one row of a tile, whose parts its warps
 // take in turn; else a warp has a row and takes all its parts.  Maxima, sums and accumulators of eight parts are fetched at once.
-template <int D, int ROWS, int SHARED>
+// GROUP workers in a row have joined their inner parts already (kv8_attention_kernel).  CTAs are small, so that they find room as the first
+// kernel's leave: with 1024 threads instead of 256 a decode of 2 x 150001 tokens took 64 us instead of 59.
+template <int D, int ROWS, int GROUP, int SHARED>
 __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_attention_join_kernel(const Kv8AttnParams p, int records, int live) {
   constexpr int kPart = ROWS * (D + 2);
   constexpr int kW = (SHARED ? kJoinRowThreads : kJoinThreads) / 32, kA = D / 32, kBatch = 8;
@@ -204,23 +207,24 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
   const int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
   const int row = rec.w + r, rows = rec2.x, head = rec2.y;
   if (rec.x < 0 || row >= rows) return;  // the whole CTA where it shares a row
-  const int first = rec.x + (SHARED ? warp : 0);
+  // the parts: the first worker's, those of workers between that begin a group, the last worker's
+  const int begin = rec.x / GROUP, n = rec.y > rec.x ? (rec.y - 1) / GROUP - begin + 2 : 1;
   constexpr int kStride = SHARED ? kW : 1;
   float m = -INFINITY, l = 0.0f, a[kA];
 #pragma unroll
   for (int i = 0; i < kA; ++i) a[i] = 0.0f;
-  for (int w0 = first; w0 <= rec.y; w0 += kBatch * kStride) {
+  for (int i0 = SHARED ? warp : 0; i0 < n; i0 += kBatch * kStride) {
     float pm[kBatch], pl[kBatch], x[kBatch][kA];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int w = w0 + j * kStride;
+      const int k = i0 + j * kStride;
       pm[j] = -INFINITY;
       pl[j] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kA; ++i) x[j][i] = 0.0f;
-      if (w <= rec.y) {
+      if (k < n) {
         // the first part is its worker's last tile, the others are their workers' first
-        const float* q = p.parts + (size_t)(2 * w + (w == rec.x ? 1 : 0)) * kPart;
+        const float* q = p.parts + (size_t)(k == 0 ? 2 * rec.x + 1 : 2 * (k == n - 1 ? rec.y : (begin + k) * GROUP)) * kPart;
         pm[j] = __ldcg(q + r);
         pl[j] = __ldcg(q + ROWS + r);
         q += 2 * ROWS + r * D + lane * kA;
@@ -281,13 +285,13 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
 }
 
 // Few tiles are split into many parts each: a CTA for each of their rows.
-template <int D, int ROWS>
+template <int D, int ROWS, int GROUP>
 int launch_join(const Kv8AttnParams& ap, const Kv8AttnPlan& pl, const DeviceInfo* dev, cudaStream_t s) {
   const unsigned rows = (unsigned)pl.records * pl.live;
   if (rows <= 2u * dev->sm_count)
-    return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 1>, dim3(rows), kJoinRowThreads, 0, s, ap, pl.records, pl.live);
+    return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, GROUP, 1>, dim3(rows), kJoinRowThreads, 0, s, ap, pl.records, pl.live);
   constexpr unsigned kRows = kJoinThreads / 32;
-  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, 0>, dim3((rows + kRows - 1) / kRows), kJoinThreads, 0, s, ap,
+  return launch_early("kv8_attention_join_kernel", kv8_attention_join_kernel<D, ROWS, GROUP, 0>, dim3((rows + kRows - 1) / kRows), kJoinThreads, 0, s, ap,
                       pl.records, pl.live);
 }
 

@@ -31,7 +31,7 @@ namespace liger {
 namespace {
 
 constexpr int kBlock = 128;         // keys of a block, rows of a half
-constexpr int kItemRows = 256;
+constexpr int kItemRows = kTcRows;
 constexpr int kItemCost = 1;        // what it costs to begin a tile, in blocks (fitted to the CTAs' times: 1.5)
 constexpr int kMinPlaces = 4;       // places that are worth a CTA
 constexpr int kSoftmaxWarps = 16, kCodeWarps = 8, kQueryWarps = 2;
@@ -224,7 +224,7 @@ struct Walk {
     b = sh.b[0];
     e = load_entry(p, b, false);
     const long long inside = at - sh.first[0], per = head_places(p, e);
-    head = (int)(inside / per);
+    head = min((int)(inside / per), p.c.kv_heads - 1);
     long long rest = inside % per;
     rt = 0;
     for (;;) {
@@ -843,7 +843,7 @@ int launch(const Kv8AttnParams& p, const Kv8AttnPlan& pl, const DeviceInfo* dev,
   int rc = allow_smem(kv8_attention_tc_kernel<D, TYPE>, Cfg<D>::kSmem, dev, allowed);
   if (rc != LIGER_OK) return rc;
   rc = launch_early("kv8_attention_tc_kernel", kv8_attention_tc_kernel<D, TYPE>, dim3(pl.workers), kThreads, Cfg<D>::kSmem, s, p);
-  return rc != LIGER_OK ? rc : launch_join<D, kItemRows>(p, pl, dev, s);
+  return rc != LIGER_OK ? rc : launch_join<D, kItemRows, 1>(p, pl, dev, s);
 }
 
 }  // namespace
