@@ -578,7 +578,10 @@ Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a,
   p.workers = tc ? ctas : ctas * kWarps;
   p.by_tile = tiles * a->batch <= p.workers;
   p.records = p.by_tile ? p.tiles * a->batch : p.workers;
-  p.bytes = p.whole ? 0 : (size_t)p.workers * sizeof(Kv8Record) + (size_t)2 * p.workers * p.rows * (c->head_dim + 2) * sizeof(float);
+  auto bytes_of = [&](int workers, int rows) { return (size_t)workers * (sizeof(Kv8Record) + (size_t)2 * rows * (c->head_dim + 2) * sizeof(float)); };
+  p.bytes = p.whole ? 0 : bytes_of(p.workers, p.rows);
+  // what kv8_attention_tc_kernel takes suffices for the other one: so a call with smaller sizes never needs more
+  if (rows > kFewRows) p.bytes = bytes_of(sm_count, kTcRows);
   return p;
 }
 

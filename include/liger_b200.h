@@ -292,8 +292,8 @@ LIGER_API int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_app
  * does not exist.  A key on a page that does not exist is left out.
  *
  * scratch holds the partial results of sequences that are split over several thread blocks:
- * liger_kv8_attention_scratch_bytes() bytes (it reads the sizes in *args, not its pointers), 16-byte aligned, not shared
- * with a call that may run at the same time, captured graphs included.  ldo % 8 == 0, out and q 16-byte aligned, strides
+ * liger_kv8_attention_scratch_bytes() bytes (it reads the sizes in *args, not its pointers; a call whose sizes
+ * are no larger never needs more), 16-byte aligned, not shared with a call that may run at the same time, captured graphs included.  ldo % 8 == 0, out and q 16-byte aligned, strides
  * multiples of 8 elements.
  */
 typedef struct liger_kv8_attention_args {

@@ -138,6 +138,18 @@ def test_workspace_sizes_grow_with_what_they_are_for(liger):
     assert lib.liger_kv8_pages_scratch_bytes(C.byref(big), 4) > lib.liger_kv8_pages_scratch_bytes(C.byref(small), 4)
     assert lib.liger_kv8_pages_scratch_bytes(C.byref(small), 1000) > lib.liger_kv8_pages_scratch_bytes(C.byref(small), 4)
     assert lib.liger_kv8_pages_scratch_bytes(C.byref(small), -1) == 0
-    # attention: the pointers in the arguments are not needed
+    # attention: no call with smaller sizes needs more, so one workspace of the largest serves all
+    def need(**kw):
+        return lib.liger_kv8_attention_scratch_bytes(C.byref(wide), C.byref(attention_args(liger, ldo=1 << 20, **kw)))
+    wide = cache(liger, page_size=256, max_pages=1 << 22)
+    sizes = dict(batch=[1, 3, 40, 5000], q_len=[1, 2, 4, 5, 9, 16, 25, 100, 5000], max_kv_len=[0, 100, 1024, 1025, 100000, 1 << 25, (1 << 25) + 1, 1 << 30],
+                 heads=[4, 8, 12, 48, 256])
+    first = {n: v[1] for n, v in sizes.items()}
+    for n, v in sizes.items():
+        for other in sizes:
+            for o in sizes[other]:
+                got = [need(**{**first, other: o, n: x}) for x in v]
+                assert got == sorted(got), (n, other, o)
+    # the pointers in the arguments are not needed
     a = attention_args(liger, q=None, out=None, kv_lens=None, scratch=None)
     assert lib.liger_kv8_attention_scratch_bytes(C.byref(small), C.byref(a)) > 0
