@@ -98,13 +98,14 @@ __device__ __forceinline__ bool kv8_rows(const Kv8Entries& e, int b, int& n, int
 __device__ __forceinline__ int kv8_slot(const Kv8Entries& e, int b) { return e.slots ? kv8_ld(e.slots + b) : b; }
 
 // ---- codes ----------------------------------------------------------------------------------------------------------------
+// 1.5 * 2^23 + x: the sum's last place is 1, so the addition rounds x to a whole number (to even at ties) and leaves it in the
+// low bits.  A conversion instruction would do it at an eighth of the rate.  |x| is below 128 (kv8_append_kernel).
+constexpr float kWholeNumbers = 12582912.0f;
 // fp32 -> code, round to nearest even; e4m3 saturates, int8 wants what rounds to -127 .. 127
 template <int TYPE>
 __device__ __forceinline__ uint32_t kv8_encode4(float a, float b, float c, float d) {
   if (TYPE == LIGER_KV8_INT8) {
-    // 1.5 * 2^23 + x: the sum's last place is 1, so the addition rounds x to a whole number (to even at ties) and leaves it in
-    // the low bits.  A conversion instruction would do it at an eighth of the rate.  |x| is below 128 (kv8_append_kernel)
-    const float whole = 12582912.0f;
+    const float whole = kWholeNumbers;
     const uint32_t ia = __float_as_uint(__fadd_rn(a, whole)), ib = __float_as_uint(__fadd_rn(b, whole));
     const uint32_t ic = __float_as_uint(__fadd_rn(c, whole)), id = __float_as_uint(__fadd_rn(d, whole));
     return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);

@@ -74,7 +74,7 @@ int kv8_check_tokens(const char* what, const int* q_offsets, int batch, int q_le
 
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kMostThreads = 256;  // of a CTA
 
 struct AppendParams {
   Kv8Layer c;
@@ -83,6 +83,8 @@ struct AppendParams {
   const int* positions;
   long long batch_stride, token_stride, head_stride;
   int unit, unit_shift;  // threads of a unit: a power of two, 32 .. 256
+  int heads_shift;       // units of a CTA: neighbouring heads
+  float minus_zero;
   DeviceStatus* status;
 };
 
@@ -95,21 +97,41 @@ __device__ __forceinline__ uint32_t encode_held(const float (&f)[4], float ratio
   return kv8_encode4<TYPE>(y[0], y[1], y[2], y[3]);
 }
 
+// Eight values times the reciprocal, in pairs, and rounded (how: kv8_encode4).  The product is an fma with -0 that the compiler cannot
+// see: it would join a product and the rounding addition into one fma, which rounds once where the definition rounds twice.
 template <int TYPE>
-__device__ __forceinline__ uint2 encode_new(const uint4& x, float back) {
-  float f[8];
-  unpack8(x, f);
-  return make_uint2(kv8_encode4<TYPE>(f[0] * back, f[1] * back, f[2] * back, f[3] * back),
-                    kv8_encode4<TYPE>(f[4] * back, f[5] * back, f[6] * back, f[7] * back));
+__device__ __forceinline__ uint2 encode_new(const uint4& x, float back, float minus_zero) {
+  const uint32_t h[4] = {x.x, x.y, x.z, x.w};
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    float2 y;
+    asm("{\n\t.reg .b64 v, b, z;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\tfma.rn.f32x2 v, v, b, z;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "=f"(y.x), "=f"(y.y)
+        : "f"(f.x), "f"(f.y), "f"(back), "f"(minus_zero));
+    if (TYPE == LIGER_KV8_INT8) {
+      asm("{\n\t.reg .b64 v, b;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tadd.rn.f32x2 v, v, b;\n\tmov.b64 {%0, %1}, v;\n\t}"
+          : "+f"(y.x), "+f"(y.y)
+          : "f"(kWholeNumbers));
+      c[i] = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040);
+    } else {
+      uint16_t pair;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(y.y), "f"(y.x));
+      c[i] = pair;
+    }
+  }
+  return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
 }
 
 // Grid: (2 * groups of heads, blocks that an entry can touch, entries); a CTA has as many units of neighbouring heads, whose source
-// rows are neighbours, as fit.  No division: with one for each unit's place the kernel was bound by instructions (45 us
-// for 2048 tokens x 96 heads, now 36).
+// rows are neighbours, as fit.  Bound by HBM as to what it moves, and nearly as much by instructions: no division for a unit's place
+// (45 -> 36 us for 2256 tokens x 96 heads of 128, int8), two products or roundings in one instruction, the values' loads before the
+// table's answer is looked at, small CTAs (-> 33.8).  That is 5.1 TB/s, 78 % of the copy rate; a CTA has one phase of loads and one of stores.
 template <int D, int TYPE, int U>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kMostThreads) kv8_append_kernel(const AppendParams p) {
   constexpr int kPieces = D / 8;  // 16-byte pieces of a source row
-  __shared__ uint32_t s_max[kAppendThreads / 32];
+  __shared__ uint32_t s_max[kMostThreads / 32];
   wait_for_stream();
   const int b = blockIdx.z;
   int n, row0;
@@ -127,7 +149,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   }
   if (p.e.slots) {  // an earlier entry of the same slot that brings tokens has it
     bool dup = false;
-    for (int j = threadIdx.x; j < b; j += kAppendThreads)
+    for (int j = threadIdx.x; j < b; j += blockDim.x)
       dup |= kv8_ld(p.e.slots + j) == slot && (p.e.q_offsets == nullptr || kv8_ld(p.e.q_offsets + j + 1) > kv8_ld(p.e.q_offsets + j));
     if (__syncthreads_or(dup)) {
       if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 2, b, (unsigned)slot);
@@ -136,30 +158,16 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   }
   const int t = threadIdx.x & (p.unit - 1);
   const int is_v = blockIdx.x & 1, blk = blockIdx.y;
-  const int head = (blockIdx.x >> 1) * (kAppendThreads >> p.unit_shift) + (threadIdx.x >> p.unit_shift);
+  const int head = ((blockIdx.x >> 1) << p.heads_shift) + (threadIdx.x >> p.unit_shift);
   const int block0 = pos0 >> p.c.block_shift;            // the first block that is touched
   const int start = (block0 + blk) << p.c.block_shift;   // this unit's first position
   if (start >= pos0 + n) return;  // the whole CTA
   const bool wanted = head < p.c.kv_heads;
-  bool active = wanted;
-  int page = -1;
-  if (active) {
-    page = kv8_ld(p.c.table + (size_t)slot * p.c.max_pages + (start >> p.c.page_shift));
-    if (page < 0 || page >= p.c.num_pages) {
-      if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 3, b, (unsigned)page);
-      active = false;
-    }
-  }
-  const int inside = start & ((1 << p.c.page_shift) - 1);
-  const size_t page_head = active ? (size_t)page * p.c.kv_heads + head : 0;
+  const int page = wanted ? kv8_ld(p.c.table + (size_t)slot * p.c.max_pages + (start >> p.c.page_shift)) : -1;
   const __half* src = (is_v ? p.v : p.k) + (p.e.q_offsets ? (long long)row0 * p.token_stride : (long long)b * p.batch_stride) +
                       (long long)head * p.head_stride;
-  uint8_t* codes = (is_v ? p.c.v : p.c.k) + ((page_head << p.c.page_shift) + inside) * D;
-  float* scale = (is_v ? p.c.vs : p.c.ks) + (page_head << (p.c.page_shift - p.c.block_shift)) + (inside >> p.c.block_shift);
   const int held = pos0 - start;      // tokens that the block held before, where positive
   const int end = pos0 + n - start;   // rows [max(held, 0), end) are new
-  const bool goes_on = active && held > 0;
-  const float s_old = goes_on ? *scale : 0.0f;
 
   // the thread's pieces: piece `piece` of rows r0, r0 + rows_u, ...
   const int piece = t % kPieces, r0 = t / kPieces, rows_u = p.unit / kPieces;
@@ -182,6 +190,18 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
       }
     }
   }
+  bool active = wanted;
+  if (active && (page < 0 || page >= p.c.num_pages)) {  // asked only now, so that the values are under way before the table has answered
+    if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 3, b, (unsigned)page);
+    active = false;
+  }
+  const int inside = start & ((1 << p.c.page_shift) - 1);
+  const size_t page_head = active ? (size_t)page * p.c.kv_heads + head : 0;
+  uint8_t* codes = (is_v ? p.c.v : p.c.k) + ((page_head << p.c.page_shift) + inside) * D;
+  float* scale = (is_v ? p.c.vs : p.c.ks) + (page_head << (p.c.page_shift - p.c.block_shift)) + (inside >> p.c.block_shift);
+  const bool goes_on = active && held > 0;
+  const float s_old = goes_on ? *scale : 0.0f;
+
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const __half2* h = reinterpret_cast<const __half2*>(&x[u]);
@@ -226,12 +246,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   uint8_t* out = codes + r0 * D + piece * 8;
   if (full && finite) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) *reinterpret_cast<uint2*>(out + u * rows_u * D) = encode_new<TYPE>(x[u], back);
+    for (int u = 0; u < U; ++u) *reinterpret_cast<uint2*>(out + u * rows_u * D) = encode_new<TYPE>(x[u], back, p.minus_zero);
   } else {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = r0 + u * rows_u;
-      if (r >= held && r < r_end) *reinterpret_cast<uint2*>(out + u * rows_u * D) = finite ? encode_new<TYPE>(x[u], back) : make_uint2(0, 0);
+      if (r >= held && r < r_end) *reinterpret_cast<uint2*>(out + u * rows_u * D) = finite ? encode_new<TYPE>(x[u], back, p.minus_zero) : make_uint2(0, 0);
     }
   }
   if (t == 0) *scale = s;
@@ -239,10 +259,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
 
 template <int D, int U>
 int launch_append(const AppendParams& p, int blocks, int type, cudaStream_t stream) {
-  const int heads_cta = kAppendThreads / p.unit;
+  const int heads_cta = 1 << p.heads_shift;
   const dim3 grid(2 * ((p.c.kv_heads + heads_cta - 1) / heads_cta), blocks, p.e.batch);
   return launch_early("kv8_append_kernel", type == LIGER_KV8_INT8 ? kv8_append_kernel<D, LIGER_KV8_INT8, U> : kv8_append_kernel<D, LIGER_KV8_E4M3, U>,
-                      grid, kAppendThreads, 0, stream, p);
+                      grid, p.unit << p.heads_shift, 0, stream, p);
 }
 
 }  // namespace
@@ -272,6 +292,7 @@ extern "C" int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_ap
   p.batch_stride = a->batch_stride;
   p.token_stride = a->token_stride;
   p.head_stride = a->head_stride;
+  p.minus_zero = -0.0f;
   p.status = dev->status_dev;
   // q_len tokens that begin at the last place of a block touch this many
   const long long blocks = ((long long)a->q_len + cache->scale_block - 2) / cache->scale_block + 1;
@@ -279,6 +300,7 @@ extern "C" int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_ap
   const int pieces = cache->scale_block * (cache->head_dim / 8);
   p.unit = pieces / 8 < 32 ? 32 : pieces / 8;
   p.unit_shift = 31 - __builtin_clz(p.unit);
+  p.heads_shift = p.unit < 128 ? 7 - p.unit_shift : 0;  // 128 threads: 33.8 us; 256 take 0.9 more, 64 take 1.5 more
   cudaStream_t s = (cudaStream_t)stream;
   if (cache->head_dim == 128) return launch_append<128, 8>(p, (int)blocks, cache->type, s);
   return pieces / 8 < 32 ? launch_append<64, 4>(p, (int)blocks, cache->type, s) : launch_append<64, 8>(p, (int)blocks, cache->type, s);
