@@ -101,15 +101,26 @@ __device__ __forceinline__ void mark_owners(const int* named, int n, int limit, 
   __syncthreads();
 }
 
+// Which of the pages that a thread looks at in a round are free, bit by bit.
+__device__ __forceinline__ unsigned look_at_refs(const PagesParams& p, int base) {
+  const int at = base + (int)threadIdx.x * kLook;
+  unsigned free = 0;
+#pragma unroll
+  for (int i = 0; i < kLook; ++i) free |= (unsigned)(at + i < p.num_pages && p.refs[at + i] == 0) << i;
+  return free;
+}
+
+// The planning kernels take one trip to memory after the other (entries, counts, reference counts, table): what can be known early
+// is asked for early.
+__device__ __forceinline__ void prefetch(const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); }
+
 // The first `wanted` free pages (all, if there are fewer), lowest number first, into the workspace and, those that fit, into
-// shared memory; returns how many.
-__device__ int list_free(const PagesParams& p, int wanted, PlanShared& s) {
+// shared memory; returns how many.  `free`: of the first round.
+__device__ int list_free(const PagesParams& p, int wanted, unsigned free, PlanShared& s) {
   int found = 0;
   for (int base = 0; base < p.num_pages && found < wanted; base += kPlanThreads * kLook) {
     const int at = base + (int)threadIdx.x * kLook;
-    unsigned free = 0;
-#pragma unroll
-    for (int i = 0; i < kLook; ++i) free |= (unsigned)(at + i < p.num_pages && p.refs[at + i] == 0) << i;
+    if (base > 0) free = look_at_refs(p, base);
     int total, rank = found + block_prefix(__popc(free), total, s.warp);
 #pragma unroll
     for (int i = 0; i < kLook; ++i)
@@ -128,7 +139,7 @@ __device__ int list_free(const PagesParams& p, int wanted, PlanShared& s) {
 // the list and how many they are (-1: refused).  Entries whose pages end behind the last free one are refused.  Returns the
 // number of pages handed out.  Up to 1024 entries stay in their threads' registers.
 template <typename Want, typename Got>
-__device__ int hand_out(const PagesParams& p, PlanShared& s, Want want, Got got) {
+__device__ int hand_out(const PagesParams& p, PlanShared& s, unsigned free, Want want, Got got) {
   const long long most = (long long)p.num_pages + 1;  // more than there are: refused, whatever it is exactly
   long long ends = 0;
   int first = 0, many = -1;
@@ -143,7 +154,7 @@ __device__ int hand_out(const PagesParams& p, PlanShared& s, Want want, Got got)
       p.many[i] = many;
     }
   }
-  const int found = list_free(p, (int)min(ends, (long long)p.num_pages), s);
+  const int found = list_free(p, (int)min(ends, (long long)p.num_pages), free, s);
   int given = 0;
   for (int base = 0; base < p.n; base += kPlanThreads) {
     const int i = base + threadIdx.x;
@@ -172,10 +183,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_reserve_plan_kernel(const Pa
   extern __shared__ __align__(16) uint8_t smem_plan[];
   PlanShared& s = *reinterpret_cast<PlanShared*>(smem_plan);
   wait_for_stream();
+  const unsigned free = look_at_refs(p, 0);
+  if ((int)threadIdx.x < p.n) {
+    const int slot = p.dst[threadIdx.x];
+    if (slot >= 0 && slot < p.slots) prefetch(p.count + slot);
+    prefetch(p.lens + threadIdx.x);
+  }
   int* owner = owners_of(p, s, p.slots);
   mark_owners(p.dst, p.n, p.slots, owner);
   hand_out(
-      p, s,
+      p, s, free,
       [&](int i) {
         const int slot = p.dst[i], len = p.lens[i];
         if (slot < 0 || slot >= p.slots || len < 0) {
@@ -206,10 +223,19 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_fork_plan_kernel(const Pages
   extern __shared__ __align__(16) uint8_t smem_plan[];
   PlanShared& s = *reinterpret_cast<PlanShared*>(smem_plan);
   wait_for_stream();
+  const unsigned free = look_at_refs(p, 0);
+  if ((int)threadIdx.x < p.n) {
+    const int src = p.src[threadIdx.x], dst = p.dst[threadIdx.x], part = p.lens[threadIdx.x] / p.page_size;
+    if (dst >= 0 && dst < p.slots) prefetch(p.count + dst);
+    if (src >= 0 && src < p.slots) {
+      prefetch(p.count + src);
+      if (part >= 0 && part < p.max_pages) prefetch(p.table + (size_t)src * p.max_pages + part);
+    }
+  }
   int* owner = owners_of(p, s, p.slots);
   mark_owners(p.dst, p.n, p.slots, owner);
   const int given = hand_out(
-      p, s,
+      p, s, free,
       [&](int i) {
         const int src = p.src[i], dst = p.dst[i], len = p.lens[i];
         if (src < 0 || src >= p.slots || dst < 0 || dst >= p.slots || len < 0) {
