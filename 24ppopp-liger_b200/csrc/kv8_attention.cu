@@ -47,8 +47,8 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 // 4000 tokens, 8 heads of 128, int8 take 75 us here and 84 us in kv8_attention_tc_kernel, 64 rows 103 and 75.
 constexpr int kFewRows = 48;
 // The warps of kv8_attention_tc_kernel wait for one another over a whole tile at most, and not longer than the wait budget of 2 s: this
-// many keys take 0.3 s.  Calls whose sequences may be longer stay with this kernel, whose warps do not wait.
-constexpr int kLongTile = 1 << 25;
+// many keys take 0.5 s.  Calls whose sequences may be longer stay with this kernel, whose warps do not wait.
+constexpr int kLongTile = 1 << 24;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ROWS: of a tile, 4, 8, 16 or 24

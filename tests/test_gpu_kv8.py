@@ -248,6 +248,30 @@ def test_values_that_are_not_finite_reach_only_those_who_see_them(gpu, liger, ma
     status(gpu)
 
 
+@pytest.mark.parametrize("group", [1, 4, 6, 13, 20, 60])
+def test_a_block_that_is_not_finite_inside_a_split_sequence(gpu, liger, group):
+    """Its parts are joined inside a thread block and between thread blocks: the one head that sees it is NaN, the rest is right."""
+    lens = [9000, 8000, 500]
+    cache = Cache("int8", num_pages=280, kv_heads=2, page_size=64, scale_block=32, head_dim=128, slots=3, max_pages=160)
+    cache.give_pages(lens)
+    cache.fill(lens, spread=50.0)
+    cache.ks[0, int(cache.table[0, 70]), 1, 1] = float("nan")
+    cache.to_gpu(liger)
+    heads = 2 * group
+    q = torch.randn((3, heads, 128), generator=torch.Generator().manual_seed(8)).half()
+    dq, dl = q.cuda(), ints(lens)
+    out = torch.zeros((3, heads * 128), dtype=torch.float16, device="cuda")
+    a = attend_args(liger, cache, dq, out, dl, heads, 1, 3)
+    liger.check(gpu.liger_kv8_attention(cache.by, C.byref(a), stream_ptr()))
+    torch.cuda.synchronize()
+    got = out.cpu().view(3, heads, 128)
+    assert bool(got[0, group:].isnan().all()) and not bool(got[0, :group].isnan().any()) and not bool(got[1:].isnan().any())
+    cache.ks[0, int(cache.table[0, 70]), 1, 1] = 0.01  # the other head of sequence 0, and the other sequences
+    got[0, group:] = attention(cache, 0, q[:1], 1, lens[0], 0, 128 ** -0.5, 1)[0][0, group:].half()
+    check_attention(got.view(3, -1), cache, q, [0, 1, 2, 3], lens, [0, 1, 2], 128 ** -0.5, 1)
+    status(gpu)
+
+
 @pytest.mark.parametrize("many,group", [(1, 1), (1, 12), (3, 20)])
 def test_bad_tables_lengths_and_offsets_are_left_out(gpu, liger, many, group):
     """Numbers on the device that name nothing: the kernels leave them out, say so, and answer the rest of the call."""

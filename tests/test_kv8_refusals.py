@@ -142,7 +142,7 @@ def test_workspace_sizes_grow_with_what_they_are_for(liger):
     def need(**kw):
         return lib.liger_kv8_attention_scratch_bytes(C.byref(wide), C.byref(attention_args(liger, ldo=1 << 20, **kw)))
     wide = cache(liger, page_size=256, max_pages=1 << 22)
-    sizes = dict(batch=[1, 3, 40, 5000], q_len=[1, 2, 4, 5, 9, 16, 25, 100, 5000], max_kv_len=[0, 100, 1024, 1025, 100000, 1 << 25, (1 << 25) + 1, 1 << 30],
+    sizes = dict(batch=[1, 3, 40, 5000], q_len=[1, 2, 4, 5, 9, 16, 25, 100, 5000], max_kv_len=[0, 100, 1024, 1025, 100000, 1 << 24, (1 << 24) + 1, 1 << 30],
                  heads=[4, 8, 12, 48, 256])
     first = {n: v[1] for n, v in sizes.items()}
     for n, v in sizes.items():
