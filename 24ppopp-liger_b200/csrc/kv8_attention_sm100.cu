@@ -20,11 +20,12 @@
 // running maximum moves only when a score exceeds it by 2^8.  P is rounded to fp16 (2^-11 of each weight; with many keys the roundings average out, and in
 // the result they weigh as much as its own rounding).
 //
-// Measured: 8 prompts of up to 512 tokens behind up to 2048, 96 heads of 128, int8: 327 .. 332 us, 390 TFLOP/s.  A half's block takes some
+// Measured: 8 prompts of up to 512 tokens behind up to 2048, 96 heads of 128, int8: 306 us, 421 TFLOP/s.  A half's block takes some
 // 6400 cycles: 2000 .. 2500 until its scores are there (its O += P V and next S behind the other half's in one pipe), 1100 .. 1400
 // for the maxima, 290 for telling the other warp, 2060 for the weights (the exponentials' own rate, when both halves are at it at once).
-// Scores of 64 keys, computed one ahead, took 348 us: products of 64 columns cost as much time as those of 128.  Handing the weights
-// over in two parts changed nothing.
+// Tried before the last step (then 331 us): scores of 64 keys, computed one ahead, 348 us, since products of 64 columns cost as much time as
+// those of 128; the weights handed over in two parts, no change; weights with the maximum so far in the same pass as the new one, 356 us:
+// they have to wait in registers, and spill.
 //
 // Shares, parts and their joining: kv8_attention.cuh, a CTA being a worker and a block of 128 keys a step.
 #include <type_traits>
@@ -667,7 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
       const int s0 = w->s0, stop = h ? w->stop1 : w->stop0, all = max(w->stop0, w->stop1);
       const int rows = w->n * p.group, r = w->rt * kItemRows + r_tile;
       const int limit = r < rows ? limit_of(p, w->len, w->n, r) : 0;
-      const int limit_low = __reduce_min_sync(0xffffffffu, limit), limit_high = __reduce_max_sync(0xffffffffu, limit);
+      // rows that are not there ask for no mask: the last tile of a prompt would else take the careful way throughout (332 -> 307 us)
+      const int limit_low = __reduce_min_sync(0xffffffffu, r < rows ? limit : w->len), limit_high = __reduce_max_sync(0xffffffffu, limit);
       float m_ref = -INFINITY, l = 0.0f, ref = 1.0f;
 #pragma unroll 1
       for (int j = s0; j < stop; ++j, ++ns) {
@@ -680,8 +682,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         const int cut = limit - j * kBlock - cp * 64;  // this thread's columns from here on are not seen
         // groups of 16 columns: the first `free` are seen by all rows of the warp (none, where a page is missing or a scale is 0 or not
         // finite), those from `shut` on by none
-        const int free = rf.z == 0.0f ? min(4, (limit_low - j * kBlock - cp * 64) >> 4) : 0;
         const int shut = min(4, (limit_high - j * kBlock - cp * 64 + 15) >> 4);
+        const int free = rf.z == 0.0f ? min(shut, (limit_low - j * kBlock - cp * 64) >> 4) : 0;
         // the rows' largest scores, in log2 units and without the value scales; the two warps of a row tell each other
         float mx = -INFINITY;
 #pragma unroll 1
@@ -714,44 +716,46 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         float sum = 0.0f;
 #pragma unroll 1
         for (int gi = 0; gi < 4; ++gi) {
-          uint32_t x[16], pk[8];
-          tmem_ld_32x16(s_addr + gi * 16, x);
-          const float4 f = lds128(sc + gi * 16);
-          const float off = f.y - m_safe;
-          tmem_ld_wait16(x);
-          float total;
-          if (gi < free) {
-            const uint64_t f2 = pack2(f.x, f.x), off2 = pack2(off, off);
-            uint64_t a = 0, b = 0;
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float2 y0 = unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), f2, off2));
-              const float2 y1 = unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), f2, off2));
-              const float w0 = exp2_approx(y0.x), w1 = exp2_approx(y0.y), w2 = exp2_approx(y1.x), w3 = exp2_approx(y1.y);
-              a = add2(a, pack2(w0, w1));
-              b = add2(b, pack2(w2, w3));
-              pk[i >> 1] = pack_half2(w0, w1);
-              pk[(i >> 1) + 1] = pack_half2(w2, w3);
-            }
-            const float2 ab = unpack2(add2(a, b));
-            total = ab.x + ab.y;
-          } else if (gi >= shut) {
-            total = 0.0f;
+          uint32_t pk[8];
+          if (gi >= shut) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) pk[i] = 0;
           } else {
-            const int seen = cut - gi * 16;
-            total = 0.0f;
+            uint32_t x[16];
+            tmem_ld_32x16(s_addr + gi * 16, x);
+            const float4 f = lds128(sc + gi * 16);
+            const float off = f.y - m_safe;
+            tmem_ld_wait16(x);
+            float total;
+            if (gi < free) {
+              const uint64_t f2 = pack2(f.x, f.x), off2 = pack2(off, off);
+              uint64_t a = 0, b = 0;
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float w0 = exp2_approx(fmaf(__uint_as_float(x[i]), f.x, off)), w1 = exp2_approx(fmaf(__uint_as_float(x[i + 1]), f.x, off));
-              w0 = i < seen ? w0 : 0.0f;
-              w1 = i + 1 < seen ? w1 : 0.0f;
-              total += w0 + w1;
-              pk[i >> 1] = f.z < 0.0f ? 0u : pack_half2(w0, w1);  // values of zero scale are zeros whatever their codes are
+              for (int i = 0; i < 16; i += 4) {
+                const float2 y0 = unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), f2, off2));
+                const float2 y1 = unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), f2, off2));
+                const float w0 = exp2_approx(y0.x), w1 = exp2_approx(y0.y), w2 = exp2_approx(y1.x), w3 = exp2_approx(y1.y);
+                a = add2(a, pack2(w0, w1));
+                b = add2(b, pack2(w2, w3));
+                pk[i >> 1] = pack_half2(w0, w1);
+                pk[(i >> 1) + 1] = pack_half2(w2, w3);
+              }
+              const float2 ab = unpack2(add2(a, b));
+              total = ab.x + ab.y;
+            } else {
+              const int seen = cut - gi * 16;
+              total = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                float w0 = exp2_approx(fmaf(__uint_as_float(x[i]), f.x, off)), w1 = exp2_approx(fmaf(__uint_as_float(x[i + 1]), f.x, off));
+                w0 = i < seen ? w0 : 0.0f;
+                w1 = i + 1 < seen ? w1 : 0.0f;
+                total += w0 + w1;
+                pk[i >> 1] = f.z < 0.0f ? 0u : pack_half2(w0, w1);  // values of zero scale are zeros whatever their codes are
+              }
             }
+            sum = fmaf(total, fabsf(f.z), sum);
           }
-          sum = fmaf(total, fabsf(f.z), sum);
           tmem_st_32x8(p_addr + gi * 8, pk);
         }
         float alpha = rf.y;
