@@ -43,8 +43,9 @@ constexpr int kWholeWarps = 8;       // of a CTA that has a whole tile
 constexpr int kStep = 16;            // keys of a step
 constexpr int kTileCost = 4;         // what it costs to begin a tile, in steps
 constexpr int kMinPlaces = 8;        // places that are worth a warp
-// Rows a key head up to which this kernel is taken.  A tile has 24 at most, and the cache is read once for each: 48 rows over 12 x
-// 4000 tokens, 8 heads of 128, int8 take 75 us here and 84 us in kv8_attention_tc_kernel, 64 rows 103 and 75.
+// Rows a key head up to which this kernel is taken.  A tile has 24 at most, and the cache is read once for each.  12 x 4000 tokens, 8
+// heads, int8, here and in kv8_attention_tc_kernel: 24 rows of 128 47 and 71 us, 48 rows 76 and 73 (of 64: 57 and 63), 56 rows 103 and 73 (78
+// and 65).  At a par this one is taken, whose weights are more exact.
 constexpr int kFewRows = 48;
 // The warps of kv8_attention_tc_kernel wait for one another over a whole tile at most, and not longer than the wait budget of 2 s: this
 // many keys take 0.5 s.  Calls whose sequences may be longer stay with this kernel, whose warps do not wait.
