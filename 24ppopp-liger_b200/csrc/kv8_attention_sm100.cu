@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache for many query rows per key head (a prompt, or a chunk of one, behind what the cache
 // holds), on the tcgen05 tensor cores.
 //
-// What it cannot do without is tensor and exponential time, some 2100 cycles of either for a block of 128 keys and 256 rows.  So
+// What it cannot do without is tensor and exponential time, some 3100 and 2100 cycles for a block of 128 keys and 256 rows.  So
 // a tile has 256 rows of one key head, two halves of 128 that take turns: while the softmax of one half runs, the products
 // of the other do.  Rows are (new token, head of the group) pairs.
 //
@@ -10,20 +10,21 @@
 //     wait in registers, its pages are looked up a block before that;  one warp works out the scales of each 16 keys;
 //   two warps copy the queries of the next tile, half by half, as the last scores of this one are done;
 //   one lane issues   S = Q K^T   (128 x 128, fp32 in TMEM)   and   O += P V   with P read from TMEM;
-//   sixteen warps have half a row a thread: scores from TMEM, P = exp2 back into the place of S, as fp16; packed fp32 pairs.
+//   sixteen warps have half a row a thread: scores from TMEM, P = exp2 back into the place of S, as two fp16 parts; packed fp32 pairs.
 // With five roles on one SM the instruction cache is what is short (a first form, unrolled throughout, missed it once in 28
 // instructions and took three times as long): loops are kept rolled, and one warp walks the share for all.
 //
 // A key block's scale multiplies its columns of S in the same instruction that subtracts the maximum.  The value scale goes into
 // the exponent, w = exp2(x - m + log2(scale / reference)), so that P V needs none; the row sum takes it out again, 16 columns
 // at a time.  The reference is the first block's largest scale; O is rescaled where a block's largest leaves it by 2^6.  The
-// running maximum moves only when a score exceeds it by 2^8.  P is rounded to fp16 (2^-11 of each weight; with many keys the roundings average out, and in
-// the result they weigh as much as its own rounding).
+// running maximum moves only when a score exceeds it by 2^8.  P is a leading and a trailing fp16 part, like the other kernel's, and either is
+// multiplied with V: one part alone, 2^-11 of each weight, shows in the result as much as the result's own rounding does (relative error of the
+// prompts below 2.89e-4 instead of 2.07e-4; 305 us instead of 356).
 //
-// Measured: 8 prompts of up to 512 tokens behind up to 2048, 96 heads of 128, int8: 306 us, 421 TFLOP/s.  A half's block takes some
-// 6400 cycles: 2000 .. 2500 until its scores are there (its O += P V and next S behind the other half's in one pipe), 1100 .. 1400
-// for the maxima, 290 for telling the other warp, 2060 for the weights (the exponentials' own rate, when both halves are at it at once).
-// Tried before the last step (then 331 us): scores of 64 keys, computed one ahead, 348 us, since products of 64 columns cost as much time as
+// Measured: 8 prompts of up to 512 tokens behind up to 2048, 96 heads of 128, int8: 356 us, 361 TFLOP/s (the second product of P V not counted).  A
+// half's block took some 6400 cycles with P in one part (305 us): 2000 .. 2500 until its scores were there (its O += P V and next S behind the other
+// half's in one pipe; the second product of either half adds 512), 1100 .. 1400 for the maxima, 290 for telling the other warp, 2060 for the weights
+// (the exponentials' own rate, when both halves are at it at once).  Tried with P in one part (then 331 us): scores of 64 keys, computed one ahead, 348 us, since products of 64 columns cost as much time as
 // those of 128; the weights handed over in two parts, no change; weights with the maximum so far in the same pass as the new one, 356 us:
 // they have to wait in registers, and spill.
 //
@@ -86,10 +87,12 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 // waits for all loads so far; names the registers so that nothing uses them before
 __device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
@@ -131,6 +134,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// a and b as fp16 and what that leaves of them, as fp16 again
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t& lead, uint32_t& trail) {
+  lead = pack_half2(a, b);
+  const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&lead));
+  trail = pack_half2(a - back.x, b - back.y);
 }
 
 // ---- shared memory by 32-bit addresses: constants added to one register, where pointers would take two registers each --------------
@@ -476,8 +486,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
               if (elect_one()) {
                 const uint32_t va = sV + st * C::kTile, o = tmem + 256 + h * 128, pa = tmem + h * 128;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)  // 16 keys each; the two halves of a block's weights lie 64 columns apart
-                  umma_f16_ts(o, pa + (k >> 2) * 64 + (k & 3) * 8, v_desc(va + k * 2048), idesc_o, (j != s0 || k != 0) ? 1u : 0u);
+                for (int k = 0; k < 8; ++k) {  // 16 keys each, both parts of their weights
+                  umma_f16_ts(o, pa + k * 16, v_desc(va + k * 2048), idesc_o, (j != s0 || k != 0) ? 1u : 0u);
+                  umma_f16_ts(o, pa + k * 16 + 8, v_desc(va + k * 2048), idesc_o, 1u);
+                }
                 if (j == end - 1) bar_commit(o_full + h * 8);
               }
               __syncwarp();
@@ -648,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
     const int h = warp >> 3, cp = (warp >> 2) & 1, quad = warp & 3;
     const int r_tile = h * 128 + quad * 32 + lane, pair = h * 4 + quad;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t s_addr = tmem + h * 128 + cp * 64 + lanes, p_addr = s_addr;
+    const uint32_t s_addr = tmem + h * 128 + cp * 64 + lanes;
     const uint32_t o_addr = tmem + 256 + h * 128 + cp * (D / 2) + lanes;
     const uint32_t mine = s_pair + ((h * 2 + cp) * 128 + quad * 32 + lane) * 4, others = mine + (cp ? -512 : 512);
     uint32_t g = 0, ns = 0, no = 0, met = 0;
@@ -712,14 +724,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         mx = fmaxf(mx, lds32(others));
         const float m_try = mx > m_ref + 8.0f || m_ref == -INFINITY ? fmaxf(m_ref, mx) : m_ref;
         const float m_safe = m_try == -INFINITY ? 0.0f : m_try;
-        // the weights, 16 keys at a time; they take the place of scores that this thread has read
+        // the weights, 16 keys at a time; their leading and trailing parts take the place of the scores that they come from
         float sum = 0.0f;
 #pragma unroll 1
         for (int gi = 0; gi < 4; ++gi) {
-          uint32_t pk[8];
+          uint32_t pk[16];  // leading, trailing parts
           if (gi >= shut) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) pk[i] = 0;
+            for (int i = 0; i < 16; ++i) pk[i] = 0;
           } else {
             uint32_t x[16];
             tmem_ld_32x16(s_addr + gi * 16, x);
@@ -737,8 +749,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
                 const float w0 = exp2_approx(y0.x), w1 = exp2_approx(y0.y), w2 = exp2_approx(y1.x), w3 = exp2_approx(y1.y);
                 a = add2(a, pack2(w0, w1));
                 b = add2(b, pack2(w2, w3));
-                pk[i >> 1] = pack_half2(w0, w1);
-                pk[(i >> 1) + 1] = pack_half2(w2, w3);
+                two_parts(w0, w1, pk[i >> 1], pk[(i >> 1) + 8]);
+                two_parts(w2, w3, pk[(i >> 1) + 1], pk[(i >> 1) + 9]);
               }
               const float2 ab = unpack2(add2(a, b));
               total = ab.x + ab.y;
@@ -751,12 +763,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
                 w0 = i < seen ? w0 : 0.0f;
                 w1 = i + 1 < seen ? w1 : 0.0f;
                 total += w0 + w1;
-                pk[i >> 1] = f.z < 0.0f ? 0u : pack_half2(w0, w1);  // values of zero scale are zeros whatever their codes are
+                two_parts(f.z < 0.0f ? 0.0f : w0, f.z < 0.0f ? 0.0f : w1, pk[i >> 1], pk[(i >> 1) + 8]);  // values of zero scale are zeros whatever their codes are
               }
             }
             sum = fmaf(total, fabsf(f.z), sum);
           }
-          tmem_st_32x8(p_addr + gi * 8, pk);
+          tmem_st_32x16(s_addr + gi * 16, pk);
         }
         float alpha = rf.y;
         if (m_try != m_ref) {
