@@ -204,9 +204,20 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
   }
   wait_for_stream();
   if (at >= records) return;
-  const int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
+  int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
+  if (p.by_tile) {
+    // A worker that gave up a wait leaves no record for the tiles that it did not reach, and the workspace holds anything: what a record says
+    // about its tile is taken from the tile's number instead.  (Numbered by worker, every record is written by the launch that it belongs to.)
+    const Entry e = load_entry(p, at / p.tiles, false);
+    const int tile = at % p.tiles, tiles = row_tiles<ROWS>(p, e);
+    if (tile >= p.c.kv_heads * tiles) return;
+    rec.z = e.row0;
+    rec.w = tile % tiles * ROWS;
+    rec2 = make_int4(e.n * p.group, tile / tiles, 0, 0);
+  }
   const int row = rec.w + r, rows = rec2.x, head = rec2.y;
-  if (rec.x < 0 || row >= rows) return;  // the whole CTA where it shares a row
+  // nothing to join, or no two workers of this launch; the whole CTA where it shares a row
+  if (rec.x < 0 || rec.y <= rec.x || rec.y >= p.workers || row >= rows) return;
   // the parts: the first worker's, those of workers between that begin a group, the last worker's
   const int begin = rec.x / GROUP, n = rec.y > rec.x ? (rec.y - 1) / GROUP - begin + 2 : 1;
   constexpr int kStride = SHARED ? kW : 1;

@@ -189,6 +189,18 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t
   return __all_sync(0xffffffffu, done);
 }
 
+// Waits for products that have been issued, which end by themselves within microseconds; a million polls at most.
+__device__ __forceinline__ void bar_drain(uint32_t bar) {
+  for (uint32_t spins = 0, done = 0; !done && spins < (1u << 20); ++spins)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], 0;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar)
+        : "memory");
+}
+
 // ---- the share of a CTA, tile by tile ---------------------------------------------------------------------------------------
 struct Tile {
   int n0, n1;  // blocks that the halves see
@@ -332,7 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
   const uint32_t t_full = bars + 192, t_empty = bars + 224;   // [kTiles]
   const uint32_t tmem_slot = bars + 256, abort_flag = bars + 260;
   const uint32_t pairs = bars + 264;                          // [8]: two warps that share 32 rows
-  const uint32_t s_pair = bars + 328;                         // [maxima, sums][half][half of the keys][128 rows]
+  const uint32_t drained = bars + 328;                        // products that are under way as the CTA gives up
+  const uint32_t s_pair = bars + 336;                         // [maxima, sums][half][half of the keys][128 rows]
   __shared__ Kv8Shares<1> shares;
   __shared__ Segment segments[kTiles];
 
@@ -356,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
       bar_init(t_empty + i * 8, kThreads / 32);
     }
     for (int i = 0; i < 8; ++i) bar_init(pairs + i * 8, 2);
+    bar_init(drained, 1);
     asm volatile("st.volatile.shared.u32 [%0], 0;" ::"r"(abort_flag) : "memory");
     fence_barrier_init();
   }
@@ -849,13 +863,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
 
   tc_fence_before();
   __syncthreads();
+  uint32_t given_up;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(given_up) : "r"(abort_flag));
   if (warp == kProductWarp) {
     tc_fence_after();
+    if (given_up) {  // nobody may have waited for the last products: they end before the memory that they use goes to others
+      if (elect_one()) bar_commit(drained);
+      __syncwarp();
+      bar_drain(drained);
+    }
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }
-  uint32_t given_up;
-  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(given_up) : "r"(abort_flag));
   if (threadIdx.x == 0 && given_up) report_failure(p.status, LIGER_DEV_TIMEOUT, 0x210u, blockIdx.x, 0);
 }
 

@@ -10,6 +10,7 @@ from kv8_model import Cache, attention, attention_tolerance
 from test_gpu_kv8 import attend_args, ints, status
 
 pytestmark = pytest.mark.gpu
+TIMEOUT = 1
 
 
 def attend(gpu, liger, cache, lens, q, n, causal=1, max_len=None):
@@ -45,3 +46,46 @@ def test_values_that_cancel_show_the_weights(gpu, liger, kind, d, n):
         off = (got[b * n:(b + 1) * n].double() - want).abs()
         tol = attention_tolerance(want, mixed, size, d)
         assert bool((off <= tol).all()), f"sequence {b}: worst {float((off / tol).max()):.3g} of the tolerance"
+
+
+@pytest.fixture
+def short_waits(gpu, liger):
+    liger.check(gpu.liger_set_wait_budget_ms(1))
+    yield
+    liger.check(gpu.liger_set_wait_budget_ms(2000))
+
+
+def long_sequence_of_few_pages(liger, times, q_len, group, kv_heads=10):
+    """A sequence whose table names the same 1024 tokens `times` times over: attention without a causal mask gives what those tokens alone
+    give.  Also queries for it."""
+    cache = Cache("int8", num_pages=4, kv_heads=kv_heads, page_size=256, scale_block=128, head_dim=64, slots=1, max_pages=4 * times)
+    cache.give_pages([1024])
+    cache.fill([1024])
+    cache.table[0] = cache.table[0, :4].repeat(times)
+    cache.to_gpu(liger)
+    q = torch.randn((q_len, kv_heads * group, 64), generator=torch.Generator().manual_seed(4)).half()
+    return cache, q
+
+
+def test_waits_that_run_out_write_nothing_beside_the_result(gpu, liger, short_waits):
+    """Shares of several milliseconds with a budget of one for each wait, and a workspace that holds numbers which look like records of an
+    earlier call.  Either the call is answered, or it says that a wait ran out; memory around its rows stays as it was."""
+    cache, q = long_sequence_of_few_pages(liger, 200, q_len=160, group=16)
+    heads, width = 160, 160 * 64
+    space = torch.full((160 + 2 * 64, width), 7.0, dtype=torch.float16, device="cuda")
+    out = space[64:-64]
+    dq, dl = q.cuda(), ints([1024 * 200])
+    a = attend_args(liger, cache, dq, out, dl, heads, 160, 1, causal=0)
+    for old in (0x01010101, 3, 0x00012345):
+        a.keep.view(torch.int32).fill_(old)
+        liger.check(gpu.liger_kv8_attention(cache.by, C.byref(a), stream_ptr()))
+        torch.cuda.synchronize()
+        st = (C.c_uint * 4)()
+        code = gpu.liger_device_status(C.byref(st))
+        gpu.liger_device_status_clear()
+        assert code in (0, TIMEOUT), list(st)
+        assert bool((space[:64] == 7.0).all()) and bool((space[-64:] == 7.0).all())
+        if code == 0:
+            want, mixed, size, _ = attention(cache, 0, q, 160, 1024, 0, 64 ** -0.5, 0)
+            off = (out.cpu().double().view(160, heads, 64) - want).abs()
+            assert bool((off <= attention_tolerance(want, mixed, size, 64)).all())
