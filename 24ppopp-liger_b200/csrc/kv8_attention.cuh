@@ -197,19 +197,16 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int which = SHARED ? blockIdx.x : blockIdx.x * kW + warp;  // record and row
   const int at = which / live, r = which % live;
-  if (p.by_tile && at < records) {
-    // tiles that the entry does not have left no record (this does not hang on the first kernel, which has waited for what does)
-    const Entry e = load_entry(p, at / p.tiles, false);
-    if (at % p.tiles >= p.c.kv_heads * row_tiles<ROWS>(p, e)) records = 0;
-  }
-  wait_for_stream();
+  const int entry = at / p.tiles, tile = at % p.tiles;
+  wait_for_stream();  // also for what the call before wrote, lengths and offsets: the first kernel's wait was for itself alone
   if (at >= records) return;
   int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
   if (p.by_tile) {
     // A worker that gave up a wait leaves no record for the tiles that it did not reach, and the workspace holds anything: what a record says
     // about its tile is taken from the tile's number instead.  (Numbered by worker, every record is written by the launch that it belongs to.)
-    const Entry e = load_entry(p, at / p.tiles, false);
-    const int tile = at % p.tiles, tiles = row_tiles<ROWS>(p, e);
+    Entry e;
+    kv8_rows(p.e, entry, e.n, e.row0);
+    const int tiles = row_tiles<ROWS>(p, e);
     if (tile >= p.c.kv_heads * tiles) return;
     rec.z = e.row0;
     rec.w = tile % tiles * ROWS;
