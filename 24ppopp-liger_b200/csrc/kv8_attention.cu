@@ -47,9 +47,6 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 // heads, int8, here and in kv8_attention_tc_kernel: 24 rows of 128 47 and 71 us, 48 rows 76 and 73 (of 64: 57 and 63), 56 rows 103 and 73 (78
 // and 65).  At a par this one is taken, whose weights are more exact.
 constexpr int kFewRows = 48;
-// The warps of kv8_attention_tc_kernel wait for one another over a whole tile at most, and not longer than the wait budget of 2 s: this
-// many keys take 0.5 s.  Calls whose sequences may be longer stay with this kernel, whose warps do not wait.
-constexpr int kLongTile = 1 << 24;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ROWS: of a tile, 4, 8, 16 or 24
@@ -569,7 +566,7 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
 Kv8AttnPlan plan_of(const liger_kv8_cache* c, const liger_kv8_attention_args* a, int sm_count) {
   Kv8AttnPlan p;
   const long long rows = (long long)a->q_len * (a->heads / c->kv_heads);
-  const bool tc = rows > kFewRows && a->scale > 0.0f && a->max_kv_len <= kLongTile;
+  const bool tc = rows > kFewRows && a->scale > 0.0f;
   p.rows = tc ? kTcRows : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 24;
   p.live = (int)(rows < p.rows ? rows : p.rows);
   const long long tiles = (long long)c->kv_heads * ((rows + p.rows - 1) / p.rows);

@@ -54,7 +54,7 @@ template <int D>
 struct Cfg {
   static constexpr int kTile = D / 64 * kBox;
   static constexpr int kScaleBytes = kSlots * (8 * 16 + 16);
-  static constexpr int kSmem = 6 * kTile /* Q x2, K x2, V x2 */ + kScaleBytes + 336 + 2 * 2 * 2 * 128 * 4 + 1024;
+  static constexpr int kSmem = 6 * kTile /* Q x2, K x2, V x2 */ + kScaleBytes + 344 + 2 * 2 * 2 * 128 * 4 + 1024;
   static constexpr int kPart = kItemRows * (D + 2);
 };
 
@@ -162,9 +162,11 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
 __device__ __forceinline__ void sts128(uint32_t at, float4 v) {
   sts128(at, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
 }
-// mbar_wait_bounded for a whole warp, with one answer for all lanes and fewer registers: the clock in steps of 2^20 ns
+// mbar_wait_bounded for a whole warp, with one answer for all lanes and fewer registers: the clock in steps of 2^16 ns.  Some warps wait for
+// a whole tile, which takes as long as its keys are many; so the budget counts from the last time that the CTA's products went on (a number
+// behind the abort flag), not from the wait's begin.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t abort_at) {
-  uint32_t since = 0, done;
+  uint32_t since = 0, seen = 0, done;
   for (uint32_t spins = 1;; ++spins) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -175,12 +177,16 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t
         : "memory");
     if (done) break;
     if ((spins & 0xffu) == 0) {
-      uint32_t given_up;
+      uint32_t given_up, progress;
       asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(given_up) : "r"(abort_at));
+      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(progress) : "r"(abort_at + 4));
       if (given_up) break;
-      const uint32_t now = (uint32_t)(globaltimer_ns() >> 20) | 1u;
-      if (since == 0) since = now;
-      if (now - since > (uint32_t)(g_wait_budget_ns >> 20)) {
+      const uint32_t now = (uint32_t)(globaltimer_ns() >> 16);
+      if (spins == 0x100u || progress != seen) {
+        since = now;
+        seen = progress;
+      }
+      if (now - since > (uint32_t)(g_wait_budget_ns >> 16) + 1u) {
         asm volatile("st.volatile.shared.u32 [%0], 1;" ::"r"(abort_at) : "memory");
         break;
       }
@@ -342,10 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
   const uint32_t o_full = bars + 128, o_empty = bars + 144;
   const uint32_t sc_full = bars + 160;                        // [slots]
   const uint32_t t_full = bars + 192, t_empty = bars + 224;   // [kTiles]
-  const uint32_t tmem_slot = bars + 256, abort_flag = bars + 260;
-  const uint32_t pairs = bars + 264;                          // [8]: two warps that share 32 rows
-  const uint32_t drained = bars + 328;                        // products that are under way as the CTA gives up
-  const uint32_t s_pair = bars + 336;                         // [maxima, sums][half][half of the keys][128 rows]
+  const uint32_t tmem_slot = bars + 256, abort_flag = bars + 260, progress = bars + 264;  // of the products, for bar_wait: behind the flag
+  const uint32_t pairs = bars + 272;                          // [8]: two warps that share 32 rows
+  const uint32_t drained = bars + 336;                        // products that are under way as the CTA gives up
+  const uint32_t s_pair = bars + 344;                         // [maxima, sums][half][half of the keys][128 rows]
   __shared__ Kv8Shares<1> shares;
   __shared__ Segment segments[kTiles];
 
@@ -371,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
     for (int i = 0; i < 8; ++i) bar_init(pairs + i * 8, 2);
     bar_init(drained, 1);
     asm volatile("st.volatile.shared.u32 [%0], 0;" ::"r"(abort_flag) : "memory");
+    asm volatile("st.volatile.shared.u32 [%0], 0;" ::"r"(progress) : "memory");
     fence_barrier_init();
   }
   if (warp == kProductWarp) {
@@ -531,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           }
           if (!ok) break;
           if (elect_one()) {
+            asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(progress), "r"(n + 2u) : "memory");
             if (j >= s0) bar_commit(v_empty + (n & 1u) * 8);
             if (j + 1 < stop) bar_commit(k_empty + ((n + 1) & 1u) * 8);
           }

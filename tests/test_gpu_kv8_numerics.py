@@ -89,3 +89,23 @@ def test_waits_that_run_out_write_nothing_beside_the_result(gpu, liger, short_wa
             want, mixed, size, _ = attention(cache, 0, q, 160, 1024, 0, 64 ** -0.5, 0)
             off = (out.cpu().double().view(160, heads, 64) - want).abs()
             assert bool((off <= attention_tolerance(want, mixed, size, 64)).all())
+
+
+@pytest.mark.parametrize("times", [200, 1000])
+def test_a_short_budget_suffices_for_waits_over_long_tiles(gpu, liger, short_waits, times):
+    """The budget is for a wait in which nothing goes on: a tile of a million keys takes longer than a millisecond and is answered."""
+    cache, q = long_sequence_of_few_pages(liger, times, q_len=160 if times == 200 else 20, group=16)
+    n, heads = q.shape[:2]
+    want, mixed, size, _ = attention(cache, 0, q, n, 1024, 0, 64 ** -0.5, 0)
+    got = attend(gpu, liger, cache, [1024 * times], q, n, causal=0)
+    off = (got.double() - want).abs()
+    assert bool((off <= attention_tolerance(want, mixed, size, 64)).all())
+
+
+@pytest.mark.parametrize("group", [1, 60])
+def test_more_than_2_to_the_24_keys(gpu, liger, group):
+    cache, q = long_sequence_of_few_pages(liger, 17000, q_len=1, group=group, kv_heads=1)
+    want, mixed, size, _ = attention(cache, 0, q, 1, 1024, 0, 64 ** -0.5, 0)
+    got = attend(gpu, liger, cache, [1024 * 17000], q, 1, causal=0)
+    off = (got.double() - want).abs()
+    assert bool((off <= attention_tolerance(want, mixed, size, 64)).all())
