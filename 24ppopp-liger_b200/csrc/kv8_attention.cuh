@@ -200,19 +200,10 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
   const int entry = at / p.tiles, tile = at % p.tiles;
   wait_for_stream();  // also for what the call before wrote, lengths and offsets: the first kernel's wait was for itself alone
   if (at >= records) return;
-  int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
-  if (p.by_tile) {
-    // A worker that gave up a wait leaves no record for the tiles that it did not reach, and the workspace holds anything: what a record says
-    // about its tile is taken from the tile's number instead.  (Numbered by worker, every record is written by the launch that it belongs to.)
-    Entry e;
-    kv8_rows(p.e, entry, e.n, e.row0);
-    const int tiles = row_tiles<ROWS>(p, e);
-    if (tile >= p.c.kv_heads * tiles) return;
-    rec.z = e.row0;
-    rec.w = tile % tiles * ROWS;
-    rec2 = make_int4(e.n * p.group, tile / tiles, 0, 0);
-  }
-  const int row = rec.w + r, rows = rec2.x, head = rec2.y;
+  const int4 rec = __ldcg(reinterpret_cast<const int4*>(p.records + at)), rec2 = __ldcg(reinterpret_cast<const int4*>(p.records + at) + 1);
+  Entry e{};
+  if (p.by_tile) kv8_rows(p.e, entry, e.n, e.row0);
+  int row0 = rec.z, row = rec.w + r, rows = rec2.x, head = rec2.y;
   // nothing to join, or no two workers of this launch; the whole CTA where it shares a row
   if (rec.x < 0 || rec.y <= rec.x || rec.y >= p.workers || row >= rows) return;
   // the parts: the first worker's, those of workers between that begin a group, the last worker's
@@ -262,8 +253,20 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
     }
     m = m_new;
   }
+  if (p.by_tile) {
+    // A worker that gave up a wait leaves no record for the tiles that it did not reach, and the workspace holds anything: so what is written
+    // to follows from the tile's number.  (Numbered by worker, every record is written by the launch that it belongs to.)  Asked for early and
+  XX
+    const int tiles = row_tiles<ROWS>(p, e);
+    if (tile >= p.c.kv_heads * tiles) return;
+    row0 = e.row0;
+    row = tile % tiles * ROWS + r;
+    rows = e.n * p.group;
+    head = tile / tiles;
+    if (row >= rows) return;
+  }
   const int token = row / p.group;
-  __half* out = p.out + (size_t)(rec.z + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
+  __half* out = p.out + (size_t)(row0 + token) * p.ldo + (size_t)(head * p.group + row % p.group) * D;
   if (!SHARED) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (D == 128)
