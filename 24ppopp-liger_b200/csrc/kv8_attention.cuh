@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(SHARED ? kJoinRowThreads : kJoinThreads) kv8_a
   if (p.by_tile) {
     // A worker that gave up a wait leaves no record for the tiles that it did not reach, and the workspace holds anything: so what is written
     // to follows from the tile's number.  (Numbered by worker, every record is written by the launch that it belongs to.)  Asked for early and
-  XX
+    // looked at only here: in front of the parts it cost 0.4 us.
     const int tiles = row_tiles<ROWS>(p, e);
     if (tile >= p.c.kv_heads * tiles) return;
     row0 = e.row0;
