@@ -14,10 +14,13 @@
 // With five roles on one SM the instruction cache is what is short (a first form, unrolled throughout, missed it once in 28
 // instructions and took three times as long): loops are kept rolled, and one warp walks the share for all.
 //
-// A key block's scale multiplies its columns of S in the same instruction that subtracts the maximum.  The value scale goes into
+// A key block's scale multiplies its columns of S in the same instruction that subtracts the reference score.  The value scale goes into
 // the exponent, w = exp2(x - m + log2(scale / reference)), so that P V needs none; the row sum takes it out again, 16 columns
-// at a time.  The reference is the first block's largest scale; O is rescaled where a block's largest leaves it by 2^6.  The
-// running maximum moves only when a score exceeds it by 2^8.  P is a leading and a trailing fp16 part, like the other kernel's, and either is
+// at a time.  The reference is the first block's largest scale; O is rescaled where a block's largest leaves it (twice, a quarter).  The reference
+// score follows the blocks' largest scores up and down (kAbove, kBelow), so that a block's weights do not fall out of fp16's range because another
+// block's were larger: after a key that outweighs all others by 2^20 and whose value is small, the others make the result.  fp16 ends at 2^-24, so a weight is off by at
+// most 2^-22 of itself or 2^-28 of the block's largest weight and value scale (where the reference score is as low as it goes: 2^-52 of the largest
+// weight so far), whichever is more.  P is a leading and a trailing fp16 part, like the other kernel's, and either is
 // multiplied with V: one part alone, 2^-11 of each weight, shows in the result as much as the result's own rounding does (relative error of the
 // prompts below 2.89e-4 instead of 2.07e-4; 305 us instead of 356).
 //
@@ -48,6 +51,9 @@ constexpr int kProductWarp = kSoftmaxWarps + kCodeWarps, kScaleWarp = kProductWa
 constexpr int kThreads = 896;
 constexpr int kSoftmaxRegs = 80, kCodeRegs = 56, kProductRegs = 72;
 constexpr int kBox = 128 * 128;     // 128 rows x 64 fp16
+// Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^11, a score up to 3 above it and a value scale up to
+// twice the reference come on top.  A block's largest score is at least 6 below the reference score, unless that is 16 below the highest reference so far.
+constexpr float kUnit = 11.0f, kAbove = 3.0f, kBelow = 6.0f, kLowest = 16.0f;
 constexpr int kSlots = 4;           // scales of blocks
 
 template <int D>
@@ -605,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           float moved = 1.0f;
           if (ref == 0.0f) {
             ref = top;
-          } else if (top > ref * 64.0f || (top < ref * 0.015625f && top > ref * kScaleVanishes)) {
+          } else if (top > ref * 2.0f || (top < ref * 0.25f && top > ref * kScaleVanishes)) {
             moved = ref / top;
             ref = top;
           }
@@ -704,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
       const int limit = r < rows ? limit_of(p, w->len, w->n, r) : 0;
       // rows that are not there ask for no mask: the last tile of a prompt would else take the careful way throughout (332 -> 307 us)
       const int limit_low = __reduce_min_sync(0xffffffffu, r < rows ? limit : w->len), limit_high = __reduce_max_sync(0xffffffffu, limit);
-      float m_ref = -INFINITY, l = 0.0f, ref = 1.0f;
+      float m_ref = -INFINITY, m_top = -INFINITY, l = 0.0f, ref = 1.0f;
 #pragma unroll 1
       for (int j = s0; j < stop; ++j, ++ns) {
         const uint32_t n = g + (uint32_t)(j - s0), slot = n & 3u;
@@ -744,8 +750,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         sts32(mine, mx);
         if (!meet()) { ok = false; break; }
         mx = fmaxf(mx, lds32(others));
-        const float m_try = mx > m_ref + 8.0f || m_ref == -INFINITY ? fmaxf(m_ref, mx) : m_ref;
-        const float m_safe = m_try == -INFINITY ? 0.0f : m_try;
+        float m_try = m_ref;
+        if (mx > m_ref + kAbove || (mx < m_ref - kBelow && mx > -INFINITY)) {
+          m_try = fmaxf(mx, m_top - kLowest);
+          m_top = fmaxf(m_top, m_try);
+        }
+        const float m_safe = m_try == -INFINITY ? 0.0f : m_try - kUnit;
         // the weights, 16 keys at a time; their leading and trailing parts take the place of the scores that they come from
         float sum = 0.0f;
 #pragma unroll 1

@@ -109,3 +109,35 @@ def test_more_than_2_to_the_24_keys(gpu, liger, group):
     got = attend(gpu, liger, cache, [1024 * 17000], q, 1, causal=0)
     off = (got.double() - want).abs()
     assert bool((off <= attention_tolerance(want, mixed, size, 64)).all())
+
+
+# What a weight may be off by beside 2^-18 of itself (attention_tolerance).  Rows above 48 a key head: two fp16 parts end at 2^-24, off by 2^-25, in units
+# in which the largest weight of the call is 2^11 and those of a block of 128 keys are at most 2^6 * 4 away from that.
+def lost_in_a_block(p_top, v_top, keys=128):
+    return keys * p_top * v_top * 2.0 ** -25 * 2.0 ** -11
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("below", [17, 21, 25])
+@pytest.mark.parametrize("n", [60])
+def test_one_key_of_no_value_in_front_of_a_long_tail(gpu, liger, kind, d, below, n):
+    """The first key outweighs each of the others by 2^below, and its value is 0: what the result consists of is the tail.  Only the keys that share the
+    first one's block may lose bits to it."""
+    length = 4000
+    cache = Cache(kind, num_pages=64, kv_heads=1, page_size=64, scale_block=16, head_dim=d, slots=1, max_pages=64)
+    cache.give_pages([length])
+    k, v = torch.randn((length, 1, d), generator=cache.gen) * 0.2, 64.0 + 6.0 * torch.randn((length, 1, d), generator=cache.gen)
+    k[:, :, 0] = 0.0
+    q = torch.randn((n, 1, d), generator=torch.Generator().manual_seed(6)) * 0.2
+    q[:, :, 0] = 4.0
+    k[0, 0, 0] = below * d ** 0.5 / (4.0 * 1.4427)
+    v[0] = 0.0
+    cache.write(0, 0, k, v)
+    q = q.half()
+    got = attend(gpu, liger, cache, [length], q, n, causal=0).double()
+    want, mixed, size, top = attention(cache, 0, q, n, length, 0, d ** -0.5, 0)
+    assert 2.0 ** -9 < float(want.min()) and float(want.max()) < 8
+    tol = attention_tolerance(want, mixed, size, d) + lost_in_a_block(1.0, top)
+    off = (got - want).abs()
+    assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance, {float((off / want).max()):.3g} of the result"
