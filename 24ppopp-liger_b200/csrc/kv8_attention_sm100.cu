@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
         if (stop <= s0) continue;
         const Lookup look{p, p.c.table + (size_t)w->slot * p.c.max_pages, w->head, w->len, stop, (1 << p.c.page_shift) - 1, lane};
         int page_now = look.valid(look.page(s0), s0, p.status, b), page_next = look.page(s0 + 1);
-        float scale_now = look.scale(page_now, s0), ref = 0.0f;
+        float scale_now = look.scale(page_now, s0), ref = 0.0f, ref_top = 0.0f;
         for (int j = s0; j < stop; ++j, ++g) {
           page_next = look.valid(page_next, j + 1, p.status, b);
           const float scale_next = look.scale(page_next, j + 1);
@@ -611,10 +611,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tc_kernel(const Kv8
           float moved = 1.0f;
           if (ref == 0.0f) {
             ref = top;
-          } else if (top > ref * 2.0f || (top < ref * 0.25f && top > ref * kScaleVanishes)) {
+          } else if (top > ref * 2.0f || (top < ref * 0.25f && top > ref_top * kScaleVanishes)) {
             moved = ref / top;
             ref = top;
           }
+          ref_top = fmaxf(ref_top, ref);
           const float base = ref > 0.0f ? ref : 1.0f;
           const bool vanishes = page_now >= 0 && vs <= base * kScaleVanishes;
           if (lane < 8)

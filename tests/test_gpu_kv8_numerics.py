@@ -141,3 +141,23 @@ def test_one_key_of_no_value_in_front_of_a_long_tail(gpu, liger, kind, d, below,
     tol = attention_tolerance(want, mixed, size, d) + lost_in_a_block(1.0, top)
     off = (got - want).abs()
     assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance, {float((off / want).max()):.3g} of the result"
+
+
+@pytest.mark.parametrize("n", [60])
+@pytest.mark.parametrize("falling", [True, False])
+def test_value_scales_that_fall_or_rise_step_by_step(gpu, liger, n, falling):
+    """Values of one sign, the later blocks' 2^-59.9 and 2^-119.8 of the first ones', or the other way round: the result is the largest blocks' share, a
+    number.  One tile is one share here, so that all of a row's blocks follow one another."""
+    scales = [0.5] * 4 + [0.5 * 2.0 ** -59.9, 0.5 * 2.0 ** -119.8]
+    kv_heads, length = 200, 128 * len(scales)
+    cache = Cache("int8", num_pages=len(scales), kv_heads=kv_heads, page_size=128, scale_block=128, head_dim=64, slots=1, max_pages=len(scales))
+    cache.give_pages([length])
+    cache.fill([length])
+    cache.v.random_(60, 128, generator=cache.gen)
+    for j, scale in enumerate(scales if falling else scales[::-1]):
+        cache.vs[0, int(cache.table[0, j])] = scale
+    q = (torch.randn((n, kv_heads, 64), generator=torch.Generator().manual_seed(6))).half()
+    got = attend(gpu, liger, cache, [length], q, n, causal=0).double()
+    want, mixed, size, top = attention(cache, 0, q, n, length, 0, 64 ** -0.5, 0)
+    tol = attention_tolerance(want, mixed, size, 64) + lost_in_a_block(1.0, top)
+    assert bool(((got - want).abs() <= tol).all())
