@@ -10,12 +10,14 @@
 //                            P^T comes out of the S^T accumulators by an 8x8 transpose (movmatrix).
 //
 // Rows are (new token, head of the group) pairs, 4, 8, 16 or 24 of them a tile.  Scales: S is multiplied by its key block's scale in
-// fp32.  The value scale goes into P: w = p * (scale / reference), where the reference follows the scales in powers of
-// 16 (the accumulators are rescaled when it moves), so that w stays where fp16 is precise.  P is split into a leading and a
+// fp32.  The value scale goes into P: w = p * (scale / reference), where the reference follows the scales (the accumulators are rescaled
+// when it moves), so that w stays where fp16 is precise.  P is split into a leading and a
 // trailing fp16 part, two products, so that its rounding does not show in the result.  With at most 4 rows both parts go into one product: columns 4 .. 7
 // are the rows again, with the trailing parts.  (The GPU runs into its power limit here, 1000 W, and the products are what can be saved:
-// 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The running
-// maximum is moved only when some score exceeds it by 2^8, which a warp finds with one vote.
+// 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The reference
+// score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with one
+// reduction: so a step's weights do not fall out of fp16's range because another step's were larger.  fp16 ends at 2^-24: a weight is off by at most 2^-22 of
+// itself or 2^-25 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-53 of the largest weight so far).
 //
 // Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
@@ -48,6 +50,9 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 // and 65).  At a par this one is taken, whose weights are more exact.
 constexpr int kFewRows = 48;
 constexpr float kLog2e = 1.4426950408889634f;
+// Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^12, a score up to 2 above it and a value scale up to
+// twice the reference come on top.  A step's largest score is at least 8 below the reference score, unless that is 16 below the highest so far.
+constexpr float kUnit = 12.0f, kAbove = 2.0f, kBelow = 8.0f, kLowest = 16.0f;
 
 // ROWS: of a tile, 4, 8, 16 or 24
 template <int D, int ROWS, int WHOLE>
@@ -168,6 +173,7 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
     // this lane's rows: as B operand row g of each n-tile, as accumulator column 2t, 2t + 1
     uint32_t qf[NT][kKk][2];
     int limit[NT][2], limit_min = e.len;
+    uint32_t idle = 0;  // columns without a row, bit by bit
     auto load_rows = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -194,6 +200,7 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int rc = row_base + nt * 8 + (2 * t + c) % kCols;
+          if (rc >= rows) idle |= 1u << (nt * 8 + 2 * t + c);
           limit[nt][c] = rc >= rows ? 0 : p.causal ? min(e.len, max(0, e.len - e.n + rc / p.group + 1)) : e.len;
         }
       }
@@ -273,11 +280,11 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
         q_bias[nt][1] = -128.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
       }
     }
-    float m_ref[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f;
+    float m_ref[NT][2], m_top[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f;  // m_ref: a reference score less kUnit; m_top: the highest so far
     float o[NT][kKk][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
+      m_ref[nt][0] = m_ref[nt][1] = m_top[nt][0] = m_top[nt][1] = -INFINITY;
       l_run[nt][0] = l_run[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kKk; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f; }
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
         }
         // scores in units of log2; s[.][0], [1]: key g, rows 2t, 2t + 1; s[.][2], [3]: key g + 8
         const float xs = ks * p.scale_log2, xm = TYPE == LIGER_KV8_INT8 ? xs * 16777216.0f : xs;
-        bool grow = false;
+        uint32_t near = idle, grow = 0;  // columns whose largest score is not too far below the reference / some score is too far above
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -336,9 +343,14 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
             for (int c = 0; c < 4; ++c)
               if (key0 + g + (c >> 1) * 8 >= limit[nt][c & 1]) s[nt][c] = -INFINITY;
           }
-          grow |= fmaxf(s[nt][0], s[nt][2]) > m_ref[nt][0] + 8.0f || fmaxf(s[nt][1], s[nt][3]) > m_ref[nt][1] + 8.0f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float above = fmaxf(s[nt][c], s[nt][c + 2]) - m_ref[nt][c];
+            if (above > kUnit + kAbove) grow = 1u << 31;
+            if (above >= kUnit - kBelow) near |= 1u << (nt * 8 + 2 * t + c);
+          }
         }
-        if (__any_sync(0xffffffffu, grow)) {
+        if (__reduce_or_sync(0xffffffffu, near | grow) != (1u << (NT * 8)) - 1u) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -347,9 +359,11 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              if (mx > m_ref[nt][c]) {
-                const float alpha = exp2_approx(m_ref[nt][c] - mx);  // 0 the first time
-                m_ref[nt][c] = mx;
+              if (mx > m_ref[nt][c] + (kUnit + kAbove) || (mx < m_ref[nt][c] + (kUnit - kBelow) && mx > -INFINITY)) {
+                const float to = fmaxf(mx - kUnit, m_top[nt][c] - kLowest);
+                const float alpha = exp2_approx(m_ref[nt][c] - to);  // 0 the first time
+                m_ref[nt][c] = to;
+                m_top[nt][c] = fmaxf(m_top[nt][c], to);
                 l_run[nt][c] *= alpha;
 #pragma unroll
                 for (int d = 0; d < kKk; ++d) { o[nt][d][c] *= alpha; o[nt][d][c + 2] *= alpha; }
@@ -357,9 +371,9 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
             }
           }
         }
-        // weights.  The value scale relative to the reference; the reference moves by powers of 16
+        // weights.  The value scale relative to the reference, which moves where a scale leaves it (twice, a 16th)
         float rel = vs * v_back;
-        if (!(rel <= 16.0f && rel >= 0.0625f) && vs > fmaxf(v_ref * kScaleVanishes, FLT_MIN)) {
+        if (!(rel <= 2.0f && rel >= 0.0625f) && vs > fmaxf(v_ref * kScaleVanishes, FLT_MIN)) {
           const float back = v_ref / vs;  // 0 the first time
           v_ref = vs;
           v_back = 1.0f / vs;

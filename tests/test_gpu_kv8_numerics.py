@@ -111,8 +111,9 @@ def test_more_than_2_to_the_24_keys(gpu, liger, group):
     assert bool((off <= attention_tolerance(want, mixed, size, 64)).all())
 
 
-# What a weight may be off by beside 2^-18 of itself (attention_tolerance).  Rows above 48 a key head: two fp16 parts end at 2^-24, off by 2^-25, in units
-# in which the largest weight of the call is 2^11 and those of a block of 128 keys are at most 2^6 * 4 away from that.
+# What weights may be off by beside 2^-18 of each (attention_tolerance): two fp16 parts end at 2^-24, off by 2^-25, in units in which a weight at the
+# reference score is 2^11 (2^12 with up to 48 rows a key head) and the reference score is no higher than the largest score of the block, of 128 keys (16),
+# where that is the largest so far.
 def lost_in_a_block(p_top, v_top, keys=128):
     return keys * p_top * v_top * 2.0 ** -25 * 2.0 ** -11
 
@@ -120,7 +121,7 @@ def lost_in_a_block(p_top, v_top, keys=128):
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("below", [17, 21, 25])
-@pytest.mark.parametrize("n", [60])
+@pytest.mark.parametrize("n", [1, 7, 12, 20, 60])
 def test_one_key_of_no_value_in_front_of_a_long_tail(gpu, liger, kind, d, below, n):
     """The first key outweighs each of the others by 2^below, and its value is 0: what the result consists of is the tail.  Only the keys that share the
     first one's block may lose bits to it."""
