@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
         q_bias[nt][1] = -128.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
       }
     }
-    float m_ref[NT][2], m_top[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f;  // m_ref: a reference score less kUnit; m_top: the highest so far
+    float m_ref[NT][2], m_top[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f, v_top = 0.0f;  // m_ref: a reference score less kUnit; m_top: the highest so far
     float o[NT][kKk][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -373,9 +373,10 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
         }
         // weights.  The value scale relative to the reference, which moves where a scale leaves it (twice, a 16th)
         float rel = vs * v_back;
-        if (!(rel <= 2.0f && rel >= 0.0625f) && vs > fmaxf(v_ref * kScaleVanishes, FLT_MIN)) {
+        if (!(rel <= 2.0f && rel >= 0.0625f) && vs > fmaxf(v_top * kScaleVanishes, FLT_MIN)) {
           const float back = v_ref / vs;  // 0 the first time
           v_ref = vs;
+          v_top = fmaxf(v_top, vs);
           v_back = 1.0f / vs;
           rel = 1.0f;
 #pragma unroll

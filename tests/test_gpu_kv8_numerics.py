@@ -144,6 +144,26 @@ def test_one_key_of_no_value_in_front_of_a_long_tail(gpu, liger, kind, d, below,
     assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance, {float((off / want).max()):.3g} of the result"
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("n,max_len", [(1, 20000), (2, 900), (7, 20000), (20, 20000)])
+@pytest.mark.parametrize("falling", [True, False])
+def test_value_scales_that_fall_or_rise_with_every_step(gpu, liger, kind, n, max_len, falling):
+    """The same with few rows, whose steps are of 16 keys: three sizes in turn."""
+    scales = [0.5, 0.5 * 2.0 ** -59.9, 0.5 * 2.0 ** -119.8]
+    length = 16 * 50
+    cache = Cache(kind, num_pages=50, kv_heads=2, page_size=16, scale_block=16, head_dim=64, slots=1, max_pages=1250)
+    cache.give_pages([length])
+    cache.fill([length])
+    cache.v.random_(60, 120, generator=cache.gen)
+    for j in range(50):
+        cache.vs[0, int(cache.table[0, j])] = scales[(j if falling else 49 - j) % 3]
+    q = (torch.randn((n, 2, 64), generator=torch.Generator().manual_seed(6))).half()
+    got = attend(gpu, liger, cache, [length], q, n, causal=0, max_len=max_len).double()
+    want, mixed, size, top = attention(cache, 0, q, n, length, 0, 64 ** -0.5, 0)
+    tol = attention_tolerance(want, mixed, size, 64) + lost_in_a_block(1.0, top)
+    assert bool(((got - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("n", [60])
 @pytest.mark.parametrize("falling", [True, False])
 def test_value_scales_that_fall_or_rise_step_by_step(gpu, liger, n, falling):
