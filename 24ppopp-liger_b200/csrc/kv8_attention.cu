@@ -15,9 +15,9 @@
 // trailing fp16 part, two products, so that its rounding does not show in the result.  With at most 4 rows both parts go into one product: columns 4 .. 7
 // are the rows again, with the trailing parts.  (The GPU runs into its power limit here, 1000 W, and the products are what can be saved:
 // 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The reference
-// score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with one
-// reduction: so a step's weights do not fall out of fp16's range because another step's were larger.  fp16 ends at 2^-24: a weight is off by at most 2^-22 of
-// itself or 2^-25 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-53 of the largest weight so far).
+// score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with two votes:
+// so a step's weights do not fall out of fp16's range because another step's were larger.  fp16 ends at 2^-24: a weight is off by at most 2^-22 of
+// itself or 2^-23 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-51 of the largest weight so far).
 //
 // Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
@@ -50,9 +50,9 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 // and 65).  At a par this one is taken, whose weights are more exact.
 constexpr int kFewRows = 48;
 constexpr float kLog2e = 1.4426950408889634f;
-// Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^12, a score up to 2 above it and a value scale up to
+// Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^10, a score up to 4 above it and a value scale up to
 // twice the reference come on top.  A step's largest score is at least 8 below the reference score, unless that is 16 below the highest so far.
-constexpr float kUnit = 12.0f, kAbove = 2.0f, kBelow = 8.0f, kLowest = 16.0f;
+constexpr float kUnit = 10.0f, kAbove = 4.0f, kBelow = 8.0f, kLowest = 16.0f;
 
 // ROWS: of a tile, 4, 8, 16 or 24
 template <int D, int ROWS, int WHOLE>
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
         }
         // scores in units of log2; s[.][0], [1]: key g, rows 2t, 2t + 1; s[.][2], [3]: key g + 8
         const float xs = ks * p.scale_log2, xm = TYPE == LIGER_KV8_INT8 ? xs * 16777216.0f : xs;
-        uint32_t near = idle, grow = 0;  // columns whose largest score is not too far below the reference / some score is too far above
+        float top = -INFINITY, low = INFINITY;  // of the lane's columns, each by its two keys; a column without a reference or a score is no number and drops out
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -346,11 +346,22 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const float above = fmaxf(s[nt][c], s[nt][c + 2]) - m_ref[nt][c];
-            if (above > kUnit + kAbove) grow = 1u << 31;
-            if (above >= kUnit - kBelow) near |= 1u << (nt * 8 + 2 * t + c);
+            top = fmaxf(top, above);
+            low = fminf(low, above);
           }
         }
-        if (__reduce_or_sync(0xffffffffu, near | grow) != (1u << (NT * 8)) - 1u) {
+        // Some score is too far above its reference, or a lane has none near it; in the second case a column may still have one in another lane.
+        bool leaves = __any_sync(0xffffffffu, top > kUnit + kAbove);
+        if (!leaves && __any_sync(0xffffffffu, low < kUnit - kBelow)) {
+          uint32_t near = idle;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (fmaxf(s[nt][c], s[nt][c + 2]) - m_ref[nt][c] >= kUnit - kBelow) near |= 1u << (nt * 8 + 2 * t + c);
+          leaves = __reduce_or_sync(0xffffffffu, near) != (1u << (NT * 8)) - 1u;
+        }
+        if (leaves) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

@@ -112,7 +112,7 @@ def test_more_than_2_to_the_24_keys(gpu, liger, group):
 
 
 # What weights may be off by beside 2^-18 of each (attention_tolerance): two fp16 parts end at 2^-24, off by 2^-25, in units in which a weight at the
-# reference score is 2^11 (2^12 with up to 48 rows a key head) and the reference score is no higher than the largest score of the block, of 128 keys (16),
+# reference score is 2^11 (2^10 with up to 48 rows a key head) and the reference score is no higher than the largest score of the block, of 128 keys (16),
 # where that is the largest so far.
 def lost_in_a_block(p_top, v_top, keys=128):
     return keys * p_top * v_top * 2.0 ** -25 * 2.0 ** -11
