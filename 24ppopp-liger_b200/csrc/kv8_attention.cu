@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
           }
         }
         // Some score is too far above its reference, or a lane has none near it; in the second case a column may still have one in another lane.
-        bool leaves = __any_sync(0xffffffffu, top > kUnit + kAbove);
-        if (!leaves && __any_sync(0xffffffffu, low < kUnit - kBelow)) {
-          uint32_t near = idle;
+        bool leaves = __any_sync(0xffffffffu, top > kUnit + kAbove || low < kUnit - kBelow);
+        if (leaves) {
+          uint32_t near = top > kUnit + kAbove ? 1u << 31 : idle;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
