@@ -17,7 +17,7 @@
 // 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The reference
 // score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with two votes:
 // so a step's weights do not fall out of fp16's range because another step's were larger.  fp16 ends at 2^-24: a weight is off by at most 2^-22 of
-// itself or 2^-23 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-51 of the largest weight so far).
+// itself or 2^-23 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-74 of the row's sum so far).
 //
 // Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
@@ -51,8 +51,9 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 constexpr int kFewRows = 48;
 constexpr float kLog2e = 1.4426950408889634f;
 // Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^10, a score up to 4 above it and a value scale up to
-// twice the reference come on top.  A step's largest score is at least 8 below the reference score, unless that is 16 below the highest so far.
-constexpr float kUnit = 10.0f, kAbove = 4.0f, kBelow = 8.0f, kLowest = 16.0f;
+// twice the reference come on top.  A step's largest score is at most 8 below the reference score, unless a reference that low would make the row's
+// sum so far more than 2^50.
+constexpr float kUnit = 10.0f, kAbove = 4.0f, kBelow = 8.0f, kMostSum = 50.0f;
 
 // ROWS: of a tile, 4, 8, 16 or 24
 template <int D, int ROWS, int WHOLE>
@@ -280,11 +281,11 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
         q_bias[nt][1] = -128.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
       }
     }
-    float m_ref[NT][2], m_top[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f, v_top = 0.0f;  // m_ref: a reference score less kUnit; m_top: the highest so far
+    float m_ref[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f, v_top = 0.0f;  // m_ref: a reference score less kUnit
     float o[NT][kKk][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m_ref[nt][0] = m_ref[nt][1] = m_top[nt][0] = m_top[nt][1] = -INFINITY;
+      m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
       l_run[nt][0] = l_run[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kKk; ++i) { o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f; }
@@ -370,11 +371,14 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              float sum = l_run[nt][c];
+              sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+              sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+              sum += __shfl_xor_sync(0xffffffffu, sum, 16);
               if (mx > m_ref[nt][c] + (kUnit + kAbove) || (mx < m_ref[nt][c] + (kUnit - kBelow) && mx > -INFINITY)) {
-                const float to = fmaxf(mx - kUnit, m_top[nt][c] - kLowest);
+                const float to = fmaxf(mx - kUnit, m_ref[nt][c] - (kMostSum - __log2f(sum)));
                 const float alpha = exp2_approx(m_ref[nt][c] - to);  // 0 the first time
                 m_ref[nt][c] = to;
-                m_top[nt][c] = fmaxf(m_top[nt][c], to);
                 l_run[nt][c] *= alpha;
 #pragma unroll
                 for (int d = 0; d < kKk; ++d) { o[nt][d][c] *= alpha; o[nt][d][c + 2] *= alpha; }

@@ -181,8 +181,8 @@ __device__ __forceinline__ void find_shares(const Kv8AttnParams& p, int least, L
 }
 
 // A value scale this much below the largest so far is taken for 0: in a result of fp16 such values do not show beside it.  The accumulators are
-// in units of the reference scale, and so grow by no more than the inverse of this however often the reference moves: with 2^16 for the
-// reference score's way down, 2^15 for a weight and 2^9 for a code, 2^28 keys stay below 2^128.
+// in units of the reference scale, and so grow by no more than the inverse of this however often the reference moves.  With 2^9 for a code and sums of
+// weights below 2^50 (2^28 keys of 2^15, and 2^16 for the reference score's way down, in kv8_attention_tc_kernel 2^59 in all) they stay below 2^128.
 constexpr float kScaleVanishes = 8.6736174e-19f;  // 2^-60
 
 constexpr int kJoinRowThreads = 256, kJoinThreads = 256;
