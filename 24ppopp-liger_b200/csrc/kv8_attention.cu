@@ -17,7 +17,7 @@
 // 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The reference
 // score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with two votes:
 // so a step's weights do not fall out of fp16's range because another step's were larger.  fp16 ends at 2^-24: a weight is off by at most 2^-22 of
-// itself or 2^-23 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-74 of the row's sum so far).
+// itself or 2^-21 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-74 of the row's sum so far).
 //
 // Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
@@ -51,9 +51,9 @@ constexpr int kMinPlaces = 8;        // places that are worth a warp
 constexpr int kFewRows = 48;
 constexpr float kLog2e = 1.4426950408889634f;
 // Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^10, a score up to 4 above it and a value scale up to
-// twice the reference come on top.  A step's largest score is at most 8 below the reference score, unless a reference that low would make the row's
+// twice the reference come on top.  A step's largest score is at most 12 below the reference score, unless a reference that low would make the row's
 // sum so far more than 2^50.
-constexpr float kUnit = 10.0f, kAbove = 4.0f, kBelow = 8.0f, kMostSum = 50.0f;
+constexpr float kUnit = 10.0f, kAbove = 4.0f, kBelow = 12.0f, kMostSum = 50.0f;
 
 // ROWS: of a tile, 4, 8, 16 or 24
 template <int D, int ROWS, int WHOLE>
@@ -386,9 +386,9 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
             }
           }
         }
-        // weights.  The value scale relative to the reference, which moves where a scale leaves it (twice, a 16th)
+        // weights.  The value scale relative to the reference, which moves where a scale leaves it (twice, a quarter)
         float rel = vs * v_back;
-        if (!(rel <= 2.0f && rel >= 0.0625f) && vs > fmaxf(v_top * kScaleVanishes, FLT_MIN)) {
+        if (!(rel <= 2.0f && rel >= 0.25f) && vs > fmaxf(v_top * kScaleVanishes, FLT_MIN)) {
           const float back = v_ref / vs;  // 0 the first time
           v_ref = vs;
           v_top = fmaxf(v_top, vs);
