@@ -76,11 +76,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two key codes as the A operand of the scores: e4m3 as fp16, int8 (biased) as the low bits of subnormal fp16 numbers.
-template <int TYPE, int HIGH>
-__device__ __forceinline__ uint32_t key_pair(uint32_t w) {
-  return TYPE == LIGER_KV8_INT8 ? __byte_perm(w, 0u, HIGH ? 0x4342 : 0x4140) : kv8_pair<TYPE, HIGH>(w);
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -263,24 +258,6 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
     for (int i = 0; i < C::kStages - 1; ++i) copy_step(i);
 
     if (NT <= 2) load_rows();
-    // int8 keys enter the product as (code + 128) * 2^-24, subnormal fp16 numbers, which costs no instruction but the byte's placing;
-    // 128 times the row's sum is taken off again, in fp32
-    float q_bias[NT][2];
-    if (TYPE == LIGER_KV8_INT8) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kKk; ++i) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&qf[nt][i][0])), b2 = __half22float2(*reinterpret_cast<const __half2*>(&qf[nt][i][1]));
-          sum += (a.x + a.y) + (b2.x + b2.y);
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // row g's, in its four lanes
-        q_bias[nt][0] = -128.0f * __shfl_sync(0xffffffffu, sum, 8 * t);
-        q_bias[nt][1] = -128.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      }
-    }
     float m_ref[NT][2], l_run[NT][2], v_ref = 0.0f, v_back = 0.0f, v_top = 0.0f;  // m_ref: a reference score less kUnit
     float o[NT][kKk][4];
 #pragma unroll
@@ -327,18 +304,18 @@ __global__ void __launch_bounds__(Cfg<D, ROWS, WHOLE>::kThreads, Cfg<D, ROWS, WH
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const uint32_t a = kv8_bias<TYPE>(wa[w]), c = kv8_bias<TYPE>(wb[w]);
-            const uint32_t a0 = key_pair<TYPE, 0>(a), a2 = key_pair<TYPE, 1>(a), a1 = key_pair<TYPE, 0>(c), a3 = key_pair<TYPE, 1>(c);
+            const uint32_t a0 = kv8_pair<TYPE, 0>(a), a2 = kv8_pair<TYPE, 1>(a), a1 = kv8_pair<TYPE, 0>(c), a3 = kv8_pair<TYPE, 1>(c);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qf[nt][4 * h + w][0], qf[nt][4 * h + w][1]);
           }
         }
         // scores in units of log2; s[.][0], [1]: key g, rows 2t, 2t + 1; s[.][2], [3]: key g + 8
-        const float xs = ks * p.scale_log2, xm = TYPE == LIGER_KV8_INT8 ? xs * 16777216.0f : xs;
+        const float xs = ks * p.scale_log2;
         float top = -INFINITY, low = INFINITY;  // of the lane's columns, each by its two keys; a column without a reference or a score is no number and drops out
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[nt][c] = TYPE == LIGER_KV8_INT8 ? fmaf(s[nt][c], xm, q_bias[nt][c & 1] * xs) : s[nt][c] * xm;
+          for (int c = 0; c < 4; ++c) s[nt][c] *= xs;
           if (masked) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)

@@ -182,3 +182,38 @@ def test_value_scales_that_fall_or_rise_step_by_step(gpu, liger, n, falling):
     want, mixed, size, top = attention(cache, 0, q, n, length, 0, 64 ** -0.5, 0)
     tol = attention_tolerance(want, mixed, size, 64) + lost_in_a_block(1.0, top)
     assert bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 7, 20, 60])
+def test_blocks_whose_scale_one_key_has_set(gpu, liger, kind, d, n):
+    """One key of a block has codes of -127 and so no weight, the few others are 0 but for codes of -1 and 1 here and there; all queries are positive and
+    large.  A score is off by at most d * 2^-23 * sum |q code| of its own key, which is a thousandth of 128 * sum |q|."""
+    lens = [3, 4, 6, 9]
+    cache = Cache(kind, num_pages=8, kv_heads=1, page_size=16, scale_block=16, head_dim=d, slots=4, max_pages=2)
+    cache.give_pages(lens)
+    cache.fill(lens)
+    codes = torch.randint(-1, 2, cache.k.shape, generator=cache.gen) * (torch.rand(cache.k.shape, generator=cache.gen) < 0.2)
+    codes[:, :, :, 1] = -127 if kind == "int8" else -120
+    cache.k = codes.to(torch.int8).view(torch.uint8) if kind == "int8" else codes.float().to(torch.float8_e4m3fn).view(torch.uint8)
+    cache.ks.fill_(0.5)
+    q = (60.0 + 8.0 * torch.randn((4 * n, 1, d), generator=torch.Generator().manual_seed(9))).half()
+    scale = 1.0 / 64
+    cache.to_gpu(liger)
+    dq, dl = q.cuda(), ints(lens)
+    out = torch.zeros((4 * n, d), dtype=torch.float16, device="cuda")
+    a = attend_args(liger, cache, dq, out, dl, 1, n, 4, causal=0, scale=scale)
+    liger.check(gpu.liger_kv8_attention(cache.by, C.byref(a), stream_ptr()))
+    status(gpu)
+    got = out.cpu().double().view(4, n, 1, d)
+    for b, length in enumerate(lens):
+        mine = q[b * n:(b + 1) * n]
+        want, mixed, _, top = attention(cache, 0, mine, n, length, b, scale, 0)
+        # the largest sum |q code| of the keys that weigh; the other one weighs less than 2^-100 however its score is rounded
+        k = cache.values(0, b, length)[0][:, 0]
+        k = k[k.abs().amax(-1) < 1.0]
+        size = float((mine[:, 0].double().abs() @ k.abs().T).max()) * scale * 1.4427
+        tol = attention_tolerance(want, mixed, size, d) + lost_in_a_block(1.0, top)
+        off = (got[b] - want).abs()
+        assert bool((off <= tol).all()), f"sequence {b}: worst {float((off / tol).max()):.3g} of the tolerance"
