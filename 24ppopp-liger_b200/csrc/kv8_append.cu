@@ -88,6 +88,11 @@ struct AppendParams {
   DeviceStatus* status;
 };
 
+// Whether n tokens from position pos0 on have a place in a row of the page table.
+__device__ __forceinline__ bool fits(const Kv8Layer& c, int pos0, int n) {
+  return pos0 >= 0 && (long long)pos0 + n <= ((long long)c.max_pages << c.page_shift);
+}
+
 // Codes of a block whose scale grows.  The ratio is at most 1 (to rounding); a code -128 that somebody else wrote becomes -127.
 template <int TYPE>
 __device__ __forceinline__ uint32_t encode_held(const float (&f)[4], float ratio) {
@@ -143,14 +148,17 @@ __global__ void __launch_bounds__(kMostThreads) kv8_append_kernel(const AppendPa
     if (lead && !rows_ok) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend, b, 0);
     return;
   }
-  if (slot < 0 || slot >= p.c.slots || pos0 < 0 || (long long)pos0 + n > ((long long)p.c.max_pages << p.c.page_shift)) {
+  if (slot < 0 || slot >= p.c.slots || !fits(p.c, pos0, n)) {
     if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 1, b, (unsigned)slot);
     return;
   }
-  if (p.e.slots) {  // an earlier entry of the same slot that brings tokens has it
+  if (p.e.slots) {  // an earlier entry of the same slot that brings tokens, and is not itself left out, has it
     bool dup = false;
     for (int j = threadIdx.x; j < b; j += blockDim.x)
-      dup |= kv8_ld(p.e.slots + j) == slot && (p.e.q_offsets == nullptr || kv8_ld(p.e.q_offsets + j + 1) > kv8_ld(p.e.q_offsets + j));
+      if (kv8_ld(p.e.slots + j) == slot) {
+        int n_j, row0_j;
+        dup |= kv8_rows(p.e, j, n_j, row0_j) && n_j > 0 && fits(p.c, kv8_ld(p.positions + j), n_j);
+      }
     if (__syncthreads_or(dup)) {
       if (lead) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 2, b, (unsigned)slot);
       return;

@@ -265,8 +265,8 @@ typedef struct liger_kv8_cache {
  * of the sequence keeps its scale unless the new one is larger, and its codes are then rounded again to the larger scale.
  * code = round-to-nearest-even(fp32(x * fp32(1 / scale))), saturated.  A block of zeros has scale 0.
  * The pages have to be there (liger_kv8_reserve) and belong to the slot alone from positions[b] on (liger_kv8_fork sees
- * to that).  A slot that two entries with tokens name is written for the first of them only
- * (LIGER_DEV_BAD_INDEX).
+ * to that).  A slot that two entries with tokens name is written for the first of them only (LIGER_DEV_BAD_INDEX); an entry that
+ * is left out, because its offsets are no run of at most q_len rows or its positions do not exist, does not count.
  * Strides are multiples of 8 elements, k and v 16-byte aligned.
  */
 typedef struct liger_kv8_append_args {
