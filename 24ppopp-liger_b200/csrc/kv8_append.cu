@@ -81,6 +81,7 @@ struct AppendParams {
   Kv8Entries e;
   const __half *k, *v;
   const int* positions;
+  const int* refs;       // how many table entries name a page, or nullptr
   long long batch_stride, token_stride, head_stride;
   int unit, unit_shift;  // threads of a unit: a power of two, 32 .. 256
   int heads_shift;       // units of a CTA: neighbouring heads
@@ -202,6 +203,9 @@ __global__ void __launch_bounds__(kMostThreads) kv8_append_kernel(const AppendPa
   if (active && (page < 0 || page >= p.c.num_pages)) {  // asked only now, so that the values are under way before the table has answered
     if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 3, b, (unsigned)page);
     active = false;
+  } else if (active && p.refs && kv8_ld(p.refs + page) > 1) {  // another slot reads it, too
+    if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 4, b, (unsigned)page);
+    active = false;
   }
   const int inside = start & ((1 << p.c.page_shift) - 1);
   const size_t page_head = active ? (size_t)page * p.c.kv_heads + head : 0;
@@ -297,6 +301,7 @@ extern "C" int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_ap
   p.k = (const __half*)a->k;
   p.v = (const __half*)a->v;
   p.positions = a->positions;
+  p.refs = cache->page_refs;
   p.batch_stride = a->batch_stride;
   p.token_stride = a->token_stride;
   p.head_stride = a->head_stride;

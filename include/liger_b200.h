@@ -248,7 +248,7 @@ typedef struct liger_kv8_cache {
   float* v_scales;
   int* page_table; /* [slots, max_pages]: the pages of a slot in order, -1 behind the last one */
   int* page_count; /* [slots]: how many pages a slot holds (only for the page operators; else NULL) */
-  int* page_refs;  /* [num_pages]: how many table entries name a page, 0 = free (only for the page operators; else NULL) */
+  int* page_refs;  /* [num_pages]: how many table entries name a page, 0 = free (for the page operators and a check in append; else NULL) */
   int layers, num_pages, kv_heads, page_size, scale_block, head_dim, type;
   int slots, max_pages;
 } liger_kv8_cache;
@@ -265,7 +265,7 @@ typedef struct liger_kv8_cache {
  * of the sequence keeps its scale unless the new one is larger, and its codes are then rounded again to the larger scale.
  * code = round-to-nearest-even(fp32(x * fp32(1 / scale))), saturated.  A block of zeros has scale 0.
  * The pages have to be there (liger_kv8_reserve) and belong to the slot alone from positions[b] on (liger_kv8_fork sees
- * to that).  A slot that two entries with tokens name is written for the first of them only (LIGER_DEV_BAD_INDEX); an entry that
+ * to that): tokens for a page that page_refs says is shared are left out (LIGER_DEV_BAD_INDEX); with page_refs NULL nobody looks.  A slot that two entries with tokens name is written for the first of them only (LIGER_DEV_BAD_INDEX); an entry that
  * is left out, because its offsets are no run of at most q_len rows or its positions do not exist, does not count.
  * Strides are multiples of 8 elements, k and v 16-byte aligned.
  */

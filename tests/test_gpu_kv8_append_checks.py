@@ -54,3 +54,36 @@ def test_of_two_entries_that_count_the_first_is_written(gpu, liger):
     status(gpu, BAD_INDEX)
     append(cache, 0, 1, 20, k[3:8], v[3:8])
     same_cache(cache)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_a_page_that_two_slots_share_is_not_written(gpu, liger, kind):
+    """A branch that goes back into the part that it shares: those tokens are left out, in the pages that are its own they are written, and the other
+    branch reads what it did.  Once it has the pages for itself the same call is carried out."""
+    cache = Cache(kind, num_pages=16, kv_heads=2, page_size=32, scale_block=16, head_dim=64, slots=3, max_pages=4)
+    cache.give_pages([100])
+    cache.fill([100])
+    cache.to_gpu(liger)
+    space = torch.empty(gpu.liger_kv8_pages_scratch_bytes(cache.by, 1), dtype=torch.uint8, device="cuda")
+    args = ints([0]), ints([1]), ints([70])
+    liger.check(gpu.liger_kv8_fork(cache.by, *(C.c_void_p(t.data_ptr()) for t in args), 1, None, C.c_void_p(space.data_ptr()), space.numel(), stream_ptr()))
+    status(gpu)
+    for n in cache.NAMES:
+        getattr(cache, n).copy_(cache.dev[n].cpu())
+    shared = [int(p) for p in cache.table[1, :2]]
+    assert [int(cache.refs[p]) for p in shared] == [2, 2] and int(cache.table[0, 0]) == shared[0]
+    k, v = (torch.randn((40, 2, 64), generator=torch.Generator().manual_seed(i)).half() for i in range(2))
+    # positions 40 .. 79: 40 .. 63 lie in the second shared page, 64 .. 79 in the slot's own
+    call(gpu, liger, cache, k, v, [40], [1], [0, 40], 40, 40)
+    status(gpu, BAD_INDEX)
+    before = {n: getattr(cache, n)[0, shared[1]].clone() for n in ("k", "v", "ks", "vs")}
+    append(cache, 0, 1, 40, k, v)
+    for n, t in before.items():
+        getattr(cache, n)[0, shared[1]] = t
+    same_cache(cache)
+    gone = ints([0])
+    liger.check(gpu.liger_kv8_free(cache.by, C.c_void_p(gone.data_ptr()), 1, stream_ptr()))
+    call(gpu, liger, cache, k, v, [40], [1], [0, 40], 40, 40)
+    status(gpu)
+    append(cache, 0, 1, 40, k, v)
+    same_cache(cache)
