@@ -217,3 +217,25 @@ def test_blocks_whose_scale_one_key_has_set(gpu, liger, kind, d, n):
         tol = attention_tolerance(want, mixed, size, d) + lost_in_a_block(1.0, top)
         off = (got[b] - want).abs()
         assert bool((off <= tol).all()), f"sequence {b}: worst {float((off / tol).max()):.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("n", [1, 20, 60])
+def test_a_group_of_small_values_that_has_all_the_weight(gpu, liger, kind, n):
+    """Inside one block of 128 keys: 16 keys weigh 2^30 times as much as the others and their values are 2^-20 of the others'."""
+    length = 128
+    cache = Cache(kind, num_pages=2, kv_heads=1, page_size=128, scale_block=16, head_dim=64, slots=1, max_pages=1)
+    cache.give_pages([length])
+    k, v = torch.randn((length, 1, 64), generator=cache.gen) * 0.2, 64.0 + 6.0 * torch.randn((length, 1, 64), generator=cache.gen)
+    q = torch.randn((n, 1, 64), generator=torch.Generator().manual_seed(6)) * 0.2
+    k[:, :, 0], q[:, :, 0] = 0.0, 4.0
+    k[32:48, 0, 0] = 30 * 8 / (4.0 * 1.4427)
+    cache.write(0, 0, k, v)
+    cache.vs *= 512.0
+    cache.vs[0, int(cache.table[0, 0]), 0, 2] *= 2.0 ** -20
+    q = q.half()
+    got = attend(gpu, liger, cache, [length], q, n, causal=0).double()
+    want, mixed, size, top = attention(cache, 0, q, n, length, 0, 64 ** -0.5, 0)
+    tol = attention_tolerance(want, mixed, size, 64) + lost_in_a_block(1.0, top)
+    off = (got - want).abs()
+    assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance, {float((off / want).max()):.3g} of the result"
