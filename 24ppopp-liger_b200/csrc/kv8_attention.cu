@@ -46,8 +46,8 @@ constexpr int kStep = 16;            // keys of a step
 constexpr int kTileCost = 4;         // what it costs to begin a tile, in steps
 constexpr int kMinPlaces = 8;        // places that are worth a warp
 // Rows a key head up to which this kernel is taken.  A tile has 24 at most, and the cache is read once for each.  12 x 4000 tokens, 8
-// heads, int8, here and in kv8_attention_tc_kernel: 24 rows of 128 47 and 71 us, 48 rows 76 and 73 (of 64: 57 and 63), 56 rows 103 and 73 (78
-// and 65).  At a par this one is taken, whose weights are more exact.
+// heads, int8, here and in kv8_attention_tc_kernel: 24 rows of 128 50 and 82 us, 48 rows 83 and 86 (of 64: 63 and 77), 56 rows 114 and 87 (84
+// and 77); e4m3: 48 rows 78 and 84, 56 rows 107 and 86.
 constexpr int kFewRows = 48;
 constexpr float kLog2e = 1.4426950408889634f;
 // Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^10, a score up to 4 above it and a value scale up to

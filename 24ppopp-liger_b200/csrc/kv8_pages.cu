@@ -325,8 +325,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_compact_plan_kernel(const Pa
   }
 }
 
-// Copies the planned pages, 32 KB of one page, layer and array at a time: eight loads a thread under way, eight CTAs an SM.  600 pages of
-// 786 KB (4 layers, 12 heads of 128, 64 tokens): 163 us, 5.8 TB/s of reads and writes, 89 % of the copy rate; 16 KB at a time cost 4 us more.
+// Copies the planned pages, 32 KB of one page, layer and array at a time: eight loads a thread under way, five CTAs an SM (fork: four) at a time (of
+// the grid's eight; registers).  600 pages of 786 KB (4 layers, 12 heads of 128, 64 tokens): 163 us, 5.8 TB/s of reads and writes, 89 % of the
+// copy rate; 16 KB at a time cost 4 us more.
 __device__ __forceinline__ void move_pages(const PagesParams& p) {
   constexpr int kU = kMovePiece / (kMoveThreads * 16), kPiece = kMovePiece;
   const int moves = *p.n_moves;

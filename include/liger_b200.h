@@ -58,7 +58,8 @@ LIGER_API int liger_device_status_clear(void);
 /*
  * How long a kernel of this library waits (on an mbarrier, a peer's flag, a barrier across ranks) before it
  * gives up, sets LIGER_DEV_TIMEOUT and unwinds: 2000 ms unless set here (for the current device) or through the
- * environment variable LIGER_WAIT_BUDGET_MS (every device).  The reference has no counterpart: its kernels
+ * environment variable LIGER_WAIT_BUDGET_MS (every device).  liger_kv8_attention counts it from the last time that anything went on in
+ * the thread block.  The reference has no counterpart: its kernels
  * and NCCL's wait without limit (src/layer/func_wrapper.h:40-43).
  */
 LIGER_API int liger_set_wait_budget_ms(int milliseconds);
@@ -263,7 +264,9 @@ typedef struct liger_kv8_cache {
  *
  * A block's scale is (largest magnitude among its new values) * fp32(1 / largest code); a block that already holds tokens
  * of the sequence keeps its scale unless the new one is larger, and its codes are then rounded again to the larger scale.
- * code = round-to-nearest-even(fp32(x * fp32(1 / scale))), saturated.  A block of zeros has scale 0.
+ * code = round-to-nearest-even(fp32(x * fp32(1 / scale))), saturated.  A block of zeros has scale 0.  A block's scale never shrinks while
+ * it holds a token that is kept: after a return to an earlier position inside it (rejected drafts), one large value that was there still
+ * sets it; a block that is written from its first token gets a scale of its own again.
  * The pages have to be there (liger_kv8_reserve) and belong to the slot alone from positions[b] on (liger_kv8_fork sees
  * to that): tokens for a page that page_refs says is shared are left out (LIGER_DEV_BAD_INDEX); with page_refs NULL nobody looks.  A slot that two entries with tokens name is written for the first of them only (LIGER_DEV_BAD_INDEX); an entry that
  * is left out, because its offsets are no run of at most q_len rows or its positions do not exist, does not count.
@@ -290,6 +293,10 @@ LIGER_API int liger_kv8_append(const liger_kv8_cache* cache, const liger_kv8_app
  * to out + t * ldo + h * head_dim; rows that belong to no sequence are left as they were.  max_kv_len bounds kv_lens; it
  * decides how the work is split, and a sequence that is longer counts as empty (LIGER_DEV_BAD_INDEX), like one whose slot
  * does not exist.  A key on a page that does not exist is left out.
+ *
+ * Scores, maxima and sums are fp32.  The weights are multiplied with the values as two fp16 parts each, whatever the number of rows: a
+ * weight is off by at most 2^-22 of itself, or 2^-21 of the largest weight (and value scale) among the 128 keys of its place in the
+ * sequence, whichever is more; nothing grows with the number of keys.  A value scale 2^-60 of a larger one counts as 0.
  *
  * scratch holds the partial results of sequences that are split over several thread blocks:
  * liger_kv8_attention_scratch_bytes() bytes (it reads the sizes in *args, not its pointers; a call whose sizes
