@@ -1,6 +1,7 @@
 """How exact attention over the paged 8-bit cache is where its inputs make that hard: sums that cancel, one key that outweighs all others,
 blocks whose scale one key has set, scales far apart.  The bounds do not grow with the number of keys."""
 import ctypes as C
+import random
 
 import pytest
 import torch
@@ -13,13 +14,13 @@ pytestmark = pytest.mark.gpu
 TIMEOUT = 1
 
 
-def attend(gpu, liger, cache, lens, q, n, causal=1, max_len=None):
-    """`n` new tokens of every sequence, q [len(lens) * n, heads, D]; the result on the CPU, [len(lens) * n, heads, D]."""
+def attend(gpu, liger, cache, lens, q, n, causal=1, max_len=None, offsets=None):
+    """`n` new tokens of every sequence, or as the offsets say and `n` at most, q [tokens, heads, D]; the result on the CPU, [tokens, heads, D]."""
     rows, heads, d = q.shape
     cache.to_gpu(liger)
-    dq, dl = q.cuda(), ints(lens)
+    dq, dl, do = q.cuda(), ints(lens), ints(offsets) if offsets else None
     out = torch.full((rows, heads * d), 7.0, dtype=torch.float16, device="cuda")
-    a = attend_args(liger, cache, dq, out, dl, heads, n, len(lens), causal=causal, max_len=max_len)
+    a = attend_args(liger, cache, dq, out, dl, heads, n, len(lens), offsets=do, total=rows, causal=causal, max_len=max_len)
     liger.check(gpu.liger_kv8_attention(cache.by, C.byref(a), stream_ptr()))
     status(gpu)
     return out.cpu().view(rows, heads, d)
@@ -239,3 +240,32 @@ def test_a_group_of_small_values_that_has_all_the_weight(gpu, liger, kind, n):
     tol = attention_tolerance(want, mixed, size, 64) + lost_in_a_block(1.0, top)
     off = (got - want).abs()
     assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance, {float((off / want).max()):.3g} of the result"
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_calls_of_any_shape(gpu, liger, seed):
+    """Types, pages, blocks, groups, lengths, runs, causal or not, scores from flat to a few keys that take all, value scales far apart: all within the
+    bound of weights in two parts, with few rows and with many."""
+    rng = random.Random(seed)
+    for it in range(8):
+        kind, d, page = rng.choice(["int8", "e4m3"]), rng.choice([64, 128]), rng.choice([16, 32, 64, 128, 256])
+        block = rng.choice([b for b in (16, 32, 64, 128) if b <= page])
+        kv_heads, group, batch = rng.choice([1, 2, 3]), rng.choice([1, 2, 3, 5, 8, 13, 16, 20]), rng.randrange(1, 6)
+        longest, most = rng.choice([40, 300, 1000, 3000 if it == 0 else 700]), rng.choice([1, 1, 3, 8, 40, 150])
+        lens, many = [rng.randrange(0, longest + 1) for _ in range(batch)], [rng.randrange(0, most + 1) for _ in range(batch)]
+        causal, amplify, spread = rng.choice([0, 1]), rng.choice([0.1, 1.0, 1.0, 4.0, 12.0, 30.0]), rng.choice([1.0, 30.0, 1e4])
+        pages = -(-longest // page)
+        cache = Cache(kind, num_pages=sum(-(-n // page) for n in lens) + 1, kv_heads=kv_heads, page_size=page, scale_block=block, head_dim=d, slots=batch,
+                      max_pages=pages, seed=it)
+        cache.give_pages(lens)
+        cache.fill(lens, spread=spread)
+        heads = kv_heads * group
+        at = [sum(many[:b]) for b in range(batch + 1)]
+        q = (torch.randn((at[-1] + 2, heads, d), generator=torch.Generator().manual_seed(it)) * amplify).half()
+        got = attend(gpu, liger, cache, lens, q, max(max(many), 1), causal=causal, max_len=rng.choice([longest, pages * page]), offsets=at)
+        assert bool((got[at[-1]:] == 7.0).all())
+        for b, n in enumerate(many):
+            want, mixed, size, top = attention(cache, 0, q[at[b]:at[b + 1]], n, lens[b], b, d ** -0.5, causal)
+            tol = attention_tolerance(want, mixed, size, d) + lost_in_a_block(1.0, top)
+            off = (got[at[b]:at[b + 1]].double() - want).abs()
+            assert bool((off <= tol).all()), f"{it}: {kind} D{d} group {group} n {n} len {lens[b]} amplify {amplify}: {float((off / tol).max()):.3g} of the tolerance"
