@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kMostThreads) kv8_append_kernel(const AppendPa
   if (active && (page < 0 || page >= p.c.num_pages)) {  // asked only now, so that the values are under way before the table has answered
     if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 3, b, (unsigned)page);
     active = false;
-  } else if (active && p.refs && kv8_ld(p.refs + page) > 1) {  // another slot reads it, too
+  } else if (active && p.refs && kv8_ld(p.refs + page) > 1) {  // another slot reads it, too (to ask costs 0.2 us of a token each, 2 us of the prompts above)
     if (t == 0) report_failure(p.status, LIGER_DEV_BAD_INDEX, kKv8AtAppend + 4, b, (unsigned)page);
     active = false;
   }

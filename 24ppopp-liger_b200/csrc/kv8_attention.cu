@@ -15,9 +15,10 @@
 // trailing fp16 part, two products, so that its rounding does not show in the result.  With at most 4 rows both parts go into one product: columns 4 .. 7
 // are the rows again, with the trailing parts.  (The GPU runs into its power limit here, 1000 W, and the products are what can be saved:
 // 32 x 2049 tokens of 96 heads, e4m3, over seconds 286 us with two products, 271 us with one, 250 us for the copies alone.)  The reference
-// score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with two votes:
-// so a step's weights do not fall out of fp16's range because another step's were larger.  fp16 ends at 2^-24: a weight is off by at most 2^-22 of
-// itself or 2^-21 of the step's largest weight and value scale (where the reference score is as low as it goes: 2^-74 of the row's sum so far).
+// score follows the steps' largest scores up and down, but only where one leaves it (kAbove, kBelow), which a warp finds with one vote, and
+// a reduction where a lane has no score near it: so a step's weights do not fall out of fp16's range because another step's were larger (2 .. 3 % of
+// the calls below).  fp16 ends at 2^-24: a weight is off by at most 2^-22 of itself or 2^-21 of the step's largest weight and value scale (where the
+// reference score is as low as it goes: 2^-74 of the row's sum so far), whichever is more.
 //
 // Work is counted in places: a tile (sequence, key head, row tile) has one for each step of 16 keys and kTileCost for what
 // it costs to begin one.  All tiles' places form one line, and every warp takes an equal share of it, whatever the lengths
@@ -27,11 +28,11 @@
 // tiles give each tile to the eight warps of a CTA instead, which join in shared memory.  Either way a warp fills a ring of
 // stages of its own with 16-byte asynchronous copies.
 //
-// Measured (device time in a row of calls): 32 x 2049 tokens, 96 heads of 128, e4m3: 251 us, 6.4 TB/s (98 % of the copy rate; 271 us over
-// seconds); 48 x up to 16384 tokens, 8 heads of 128 for 64 queries, int8: 65 .. 71 us, 4.5 .. 4.9 TB/s; 2 x 150001 tokens, 4 heads of 128
-// for 20 queries, e4m3: 59 us, 5.2 TB/s.  What the shorter calls miss is some 7 us until the first codes arrive (lengths, table,
+// Measured (device time in a row of calls): 32 x 2049 tokens, 96 heads of 128, e4m3: 257 us, 6.3 TB/s (96 % of the copy rate; 277 us over
+// seconds); 48 x up to 16384 tokens, 8 heads of 128 for 64 queries, int8: 67 .. 73 us, 4.4 .. 4.8 TB/s; 2 x 150001 tokens, 4 heads of 128
+// for 20 queries, e4m3: 58 .. 62 us, 5.0 .. 5.3 TB/s.  What the shorter calls miss is some 7 us until the first codes arrive (lengths, table,
 // codes: one after the other) and some 5 us for the join.  5 drafted tokens of 12 sequences behind up to 6000, 8 heads for 32 queries, int8:
-// 42 us, 2.1 TB/s; here the work between the copies is what takes time (29 us without it): 72 products a step of 16 keys, with two warps
+// 45 us, 2.0 TB/s; here the work between the copies is what takes time (29 us without it): 72 products a step of 16 keys, with two warps
 // on a scheduler since 24 rows fill the registers.
 #include <cfloat>
 

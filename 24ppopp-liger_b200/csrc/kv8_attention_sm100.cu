@@ -17,19 +17,20 @@
 // A key block's scale multiplies its columns of S in the same instruction that subtracts the reference score.  The value scale goes into
 // the exponent, w = exp2(x - m + log2(scale / reference)), so that P V needs none; the row sum takes it out again, 16 columns
 // at a time.  The reference is the first block's largest scale; O is rescaled where a block's largest leaves it (twice, a quarter).  The reference
-// score follows the blocks' largest scores up and down (kAbove, kBelow), so that a block's weights do not fall out of fp16's range because another
-// block's were larger: after a key that outweighs all others by 2^20 and whose value is small, the others make the result.  fp16 ends at 2^-24, so a weight is off by at
-// most 2^-22 of itself or 2^-28 of the block's largest weight and value scale (where the reference score is as low as it goes: 2^-52 of the largest
-// weight so far), whichever is more.  P is a leading and a trailing fp16 part, like the other kernel's, and either is
-// multiplied with V: one part alone, 2^-11 of each weight, shows in the result as much as the result's own rounding does (relative error of the
-// prompts below 2.89e-4 instead of 2.07e-4; 305 us instead of 356).
+// score follows the blocks' largest scores up and down (kAbove, kBelow), so that a block's weights do not fall out of fp16's range because
+// another block's were larger: after a key that outweighs all others by 2^20 and whose value is small, the others make the result.  (That
+// and the spills that came with it: 356 -> 363 us for the prompts below.)  P is a leading and a trailing fp16 part, like the other kernel's,
+// and either is multiplied with V: one part alone, 2^-11 of each weight, shows in the result as much as the result's own rounding does
+// (relative error of the prompts 2.89e-4 instead of 2.07e-4, 305 us instead of 356).  fp16 ends at 2^-24, so a weight is off by at most 2^-22 of
+// itself or 2^-28 of the block's largest weight and value scale (where the reference score is as low as it goes: 2^-52 of the largest weight
+// so far), whichever is more.
 //
-// Measured: 8 prompts of up to 512 tokens behind up to 2048, 96 heads of 128, int8: 356 us, 361 TFLOP/s (the second product of P V not counted).  A
-// half's block took some 6400 cycles with P in one part (305 us): 2000 .. 2500 until its scores were there (its O += P V and next S behind the other
-// half's in one pipe; the second product of either half adds 512), 1100 .. 1400 for the maxima, 290 for telling the other warp, 2060 for the weights
-// (the exponentials' own rate, when both halves are at it at once).  Tried with P in one part (then 331 us): scores of 64 keys, computed one ahead, 348 us, since products of 64 columns cost as much time as
-// those of 128; the weights handed over in two parts, no change; weights with the maximum so far in the same pass as the new one, 356 us:
-// they have to wait in registers, and spill.
+// Measured: 8 prompts of up to 512 tokens behind up to 2048, 96 heads of 128, int8: 363 us, 355 TFLOP/s (the trailing parts' products not
+// counted).  With P in one part (305 us) a half's block took some 6400 cycles: 2000 .. 2500 until its scores were there (its O += P V and next S
+// behind the other half's in one pipe; the trailing part of either half adds 512), 1100 .. 1400 for the maxima, 290 for telling the other warp,
+// 2060 for the weights (the exponentials' own rate, when both halves are at it at once).  Tried with P in one part (then 331 us): scores of 64
+// keys, computed one ahead, 348 us, since products of 64 columns cost as much time as those of 128; the weights handed over in two halves, no
+// change; weights with the maximum so far in the same pass as the new one, 356 us: they have to wait in registers, and spill.
 //
 // Shares, parts and their joining: kv8_attention.cuh, a CTA being a worker and a block of 128 keys a step.
 #include <type_traits>
@@ -52,7 +53,7 @@ constexpr int kThreads = 896;
 constexpr int kSoftmaxRegs = 80, kCodeRegs = 56, kProductRegs = 72;
 constexpr int kBox = 128 * 128;     // 128 rows x 64 fp16
 // Where the weights lie among fp16 numbers (in log2 units): the reference score has weight 2^11, a score up to 3 above it and a value scale up to
-// twice the reference come on top.  A block's largest score is at least 6 below the reference score, unless that is 16 below the highest reference so far.
+// twice the reference come on top.  A block's largest score is at most 6 below the reference score, unless that is 16 below the highest so far.
 constexpr float kUnit = 11.0f, kAbove = 3.0f, kBelow = 6.0f, kLowest = 16.0f;
 constexpr int kSlots = 4;           // scales of blocks
 
